@@ -223,6 +223,113 @@ int sky_sample_session_frontier(sky_sample_session* s, uint32_t hop, const uint3
 int sky_sample_session_hop(sky_sample_session* s, uint32_t hop, const float* weights_device);
 int sky_sample_session_end(sky_sample_session* s, uint64_t* sampled, double* seconds);
 
+/* ---- choices from rows of a model's scores.  The samplers above choose from rows of stored weights; a sequence model that is
+ *      trained on their walks answers with a dense row of scores per walker instead: logits over the vertices (tokens) that may
+ *      come next, or over the experts that may work on it.  The reference has no counterpart.
+ *      These calls enqueue their kernels on `stream` (a hipStream_t of the current device; NULL: the null stream, on which
+ *      everything else here runs) and return: they allocate nothing, copy nothing to the host and do not wait, so a stream
+ *      that is being captured takes them.  Matrices are row-major in device memory, elements of `dtype`, aligned to the size of
+ *      an element; `row_stride` is in elements, 0 stands for as many as a row has.  Nothing behind the last row or the last
+ *      column is read or written.  rows == 0 is no error and does nothing.  At most 2^31 - 1 rows and columns. ---- */
+enum sky_dtype { SKY_F32 = 0, SKY_F16 = 1, SKY_BF16 = 2 };
+
+/* What is done to logits before a draw, in this order; every part is optional (NULL, zero).  Arrays are device arrays.
+ *   history      the ids each row has had: rows of history_stride words (0: history_columns), of which the first
+ *                history_lengths[r] (NULL: history_columns, which is also the most) count.  Ids that are not below `columns` are
+ *                passed over, so that paths as the walks leave them, filled with SKY_INVALID beforehand, are a history.
+ *     repetition[r]  an id that occurs: x > 0 ? x / repetition : x * repetition
+ *     presence[r], frequency[r]  an id that occurs n > 0 times from position history_first[r] on (NULL: 0; the length of a
+ *                    prompt that is not to count): x - (presence + frequency * n)
+ *   bias         row r adds bias_values[i] to the column bias_ids[i] for i in [bias_offsets[r], bias_offsets[r + 1]), offsets
+ *                of rows + 1 words, bias_count values in all (offsets beyond it are cut off).  Ids ascend within a row; equal
+ *                ones add up in their order, ids not below `columns` are passed over.
+ *   allowed      bit masks: allowed_rows rows of allowed_stride words (0: as many as `columns` bits take), bit c & 31 of word
+ *                c >> 5 set where column c may stay.  Row r takes mask row allowed_row[r] (a state of a grammar); SKY_INVALID:
+ *                no mask for this row; another value that is not below allowed_rows: nothing is allowed.  allowed_row NULL:
+ *                mask row r, or mask row 0 for every row if there is one only.
+ *   graph        row r may only go to the neighbours of vertex states[r * states_stride] (stride 0: 1) of this graph: a column
+ *                of the paths, or the states of a grammar whose edges lead to ids.  A state that is no vertex, as a walker's that
+ *                has stopped, allows nothing.  The graph lives on the current device (SKY_ERR_STATE otherwise).
+ * What is not allowed becomes -inf whatever it was, NaN included.  Arithmetic is fp32, rounded to `dtype` once.  `out` is
+ * `logits` itself with the same stride, or memory that does not overlap it. */
+typedef struct sky_logits_rules {
+  const uint32_t* history;
+  uint64_t history_stride;
+  uint32_t history_columns;
+  uint32_t bias_count;
+  const uint32_t* history_lengths;
+  const uint32_t* history_first;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const uint32_t* bias_offsets;
+  const uint32_t* bias_ids;
+  const float* bias_values;
+  const uint32_t* allowed;
+  uint64_t allowed_stride;
+  const uint32_t* allowed_row;
+  const sky_graph* graph;
+  const uint32_t* states;
+  uint64_t states_stride;
+  uint32_t allowed_rows;
+} sky_logits_rules;
+int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, uint32_t columns, uint64_t row_stride,
+                      const sky_logits_rules* rules, void* out, uint64_t out_stride, void* stream);
+
+/* One id of every row by chance.  Entries are ordered by logit, largest first, equal ones by column, and weigh
+ * exp((logit - largest) / temperature).  NaN and -inf are not there to be drawn; +inf counts as the largest number.
+ *   temperature[r]  NULL: 1; not above 0: the first entry of the order is taken
+ *   top_k[r]        only the first top_k of the order stay (0, NULL: all)
+ *   top_p[r]        only the shortest beginning of the order whose weight is at least top_p of what top_k left, the first entry in
+ *                   any case (NULL, 1 and more, NaN: all)
+ *   min_p[r]        only entries of weight min_p and more, the first in any case (NULL, 0: all)
+ * The id is the first of what stays whose weights, summed in that order, pass uniforms[r] (in [0, 1)) times their total;
+ * uniforms NULL: 53 bits of Philox(philox_seed; first_walker + r, step), a stream that no other call shares.
+ * tokens[r * tokens_stride] (stride 0: 1) receives it, so that a column of paths can take it, SKY_INVALID where a row has
+ * nothing to draw; logprobs[r] (may be NULL) the logarithm of its probability among what stays (-inf for such a row), kept[r] (may
+ * be NULL) how many stay.
+ * workspace: memory of the size that sky_logits_draw_workspace gives, aligned to 16 bytes, of which two calls that may run at the same
+ * time have one each (a captured graph keeps its own); NULL: every row is drawn from by one workgroup, the same ids, later where
+ * there are few rows. */
+typedef struct sky_draw_rules {
+  const float* temperature;
+  const uint32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+} sky_draw_rules;
+int sky_logits_draw_workspace(int dtype, uint32_t rows, uint32_t columns, uint64_t* bytes);
+int sky_logits_draw(const void* logits, int dtype, uint32_t rows, uint32_t columns, uint64_t row_stride,
+                    const sky_draw_rules* rules, const double* uniforms, uint64_t philox_seed, uint32_t first_walker,
+                    uint32_t step, uint32_t* tokens, uint64_t tokens_stride, float* logprobs, uint32_t* kept, void* workspace,
+                    uint64_t workspace_bytes, void* stream);
+
+/* The k best experts of every row.  score = softmax or sigmoid of the row's logits; experts compete by score + bias (bias[e],
+ * NULL: none), equal ones by their number.  With groups > 1 the experts form `groups` ranges of the same length, of which
+ * the groups_kept best stay: a group is worth its best expert, or its two best together (group_top2).  ids[r * k + j] receives
+ * the j-th best, weights[r * k + j] scale * score, with `renormalise` divided by the sum of the row's k scores; the bias has
+ * no part in the weights.  A logit of NaN or -inf closes an expert: it is not chosen, and places that find no open expert receive
+ * SKY_INVALID with weight 0; +inf counts as the largest number.  counts[e] (may be NULL) receives how often expert e was chosen
+ * (0 for all when there are no rows).
+ * At most 1,024 experts, k of at most 64, at most 64 groups (SKY_ERR_LIMIT).
+ * The backward call takes the same logits and rules, the ids, and dweights[r * k + j], the gradient with respect to the weights; it
+ * writes dlogits, of the logits' dtype, every column of every row.  The choice itself has no gradient, and so the bias has none; closed
+ * experts have 0. */
+typedef struct sky_route_rules {
+  uint32_t k;
+  uint32_t groups;
+  uint32_t groups_kept;
+  int sigmoid;
+  int group_top2;
+  int renormalise;
+  float scale;
+  const float* bias;
+} sky_route_rules;
+int sky_route_topk(const void* logits, int dtype, uint32_t rows, uint32_t experts, uint64_t row_stride,
+                   const sky_route_rules* rules, uint32_t* ids, float* weights, uint32_t* counts, void* stream);
+int sky_route_topk_backward(const void* logits, int dtype, uint32_t rows, uint32_t experts, uint64_t row_stride,
+                            const sky_route_rules* rules, const uint32_t* ids, const float* dweights, void* dlogits,
+                            uint64_t dlogits_stride, void* stream);
+
 /* ---- self-test hook: runs Philox4x32-10 on the device for n (counter, key) pairs.
  *      ctr_host[4n], key_host[2n] -> out_host[4n]. ---- */
 int sky_philox_selftest(const uint32_t* ctr_host, const uint32_t* key_host, uint32_t n, uint32_t* out_host);

@@ -16,6 +16,7 @@ INVALID = 0xFFFFFFFF
 FILL = 0xFFFFFFFF
 BIAS_STATIC, BIAS_NODE2VEC, BIAS_NODE2VEC_REJECT = 0, 1, 2
 W_UNIFORM, W_UNIT, W_LOGNORMAL = 0, 1, 2
+F32, F16, BF16 = 0, 1, 2
 
 EXPORTS = [
     "sky_last_error", "sky_version", "sky_device_malloc", "sky_device_free", "sky_memcpy_h2d", "sky_memcpy_d2h",
@@ -25,6 +26,7 @@ EXPORTS = [
     "sky_walk_offline_noalloc", "sky_walk_index_build",
     "sky_walk_online", "sky_sample_layout", "sky_sample_offline", "sky_sample_online", "sky_sample_session_begin", "sky_sample_session_frontier", "sky_sample_session_hop",
     "sky_sample_session_end", "sky_philox_selftest",
+    "sky_logits_adjust", "sky_logits_draw", "sky_logits_draw_workspace", "sky_route_topk", "sky_route_topk_backward",
     "sky_last_build_profile", "sky_set_option", "sky_graph_set_option", "sky_graph_unset_option",
 ]
 
@@ -56,6 +58,11 @@ def lib():
         L.sky_walk_offline.argtypes = [p, p, u32, u32, f32, u64] + walk_out
         L.sky_walk_online.argtypes = [p, C.c_int, f32, f32, p, u32, u32, f32, u64] + walk_out
         L.sky_sample_offline.argtypes = L.sky_sample_online.argtypes = [p, p, u32, p, u32, u64] + walk_out
+        L.sky_logits_adjust.argtypes = [p, C.c_int, u32, u32, u64, p, p, u64, p]
+        L.sky_logits_draw_workspace.argtypes = [C.c_int, u32, u32, p]
+        L.sky_logits_draw.argtypes = [p, C.c_int, u32, u32, u64, p, p, u64, u32, u32, p, u64, p, p, p, u64, p]
+        L.sky_route_topk.argtypes = [p, C.c_int, u32, u32, u64, p, p, p, p, p]
+        L.sky_route_topk_backward.argtypes = [p, C.c_int, u32, u32, u64, p, p, p, p, u64, p]
         _lib = L
     return _lib
 
@@ -384,3 +391,98 @@ def philox_selftest(ctr, key):
     out = np.zeros_like(ctr)
     _ck(lib().sky_philox_selftest(_p(ctr), _p(key), C.c_uint32(len(ctr)), _p(out)))
     return out
+
+
+# ---- choices from rows of scores.  Arrays are anything with a device address under `ptr`: a DeviceArray, or a view of another
+# library's memory; `stream` is the address of a HIP stream of the current device, None the null stream.
+def _addr(a):
+    if a is None:
+        return None
+    return a.ptr.value if isinstance(a.ptr, C.c_void_p) else a.ptr
+
+
+class _Rules(C.Structure):
+    """A rules struct that is built once and used for many calls; it keeps the arrays that it points to."""
+
+    def _point(self, arrays):
+        self._arrays = arrays
+        for name, a in arrays.items():
+            setattr(self, name, _addr(a))
+        self.ref = C.byref(self)
+
+
+class LogitsRules(_Rules):
+    """sky_logits_rules."""
+    _fields_ = [("history", C.c_void_p), ("history_stride", C.c_uint64), ("history_columns", C.c_uint32), ("bias_count", C.c_uint32),
+                ("history_lengths", C.c_void_p), ("history_first", C.c_void_p), ("repetition", C.c_void_p), ("presence", C.c_void_p),
+                ("frequency", C.c_void_p), ("bias_offsets", C.c_void_p), ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p),
+                ("allowed", C.c_void_p), ("allowed_stride", C.c_uint64), ("allowed_row", C.c_void_p), ("graph", C.c_void_p),
+                ("states", C.c_void_p), ("states_stride", C.c_uint64), ("allowed_rows", C.c_uint32)]
+
+    def __init__(self, history=None, history_columns=0, history_stride=0, history_lengths=None, history_first=None, repetition=None,
+                 presence=None, frequency=None, bias_offsets=None, bias_ids=None, bias_values=None, bias_count=0, allowed=None,
+                 allowed_rows=0, allowed_stride=0, allowed_row=None, graph=None, states=None, states_stride=0):
+        super().__init__(history_stride=history_stride, history_columns=history_columns, bias_count=bias_count,
+                         allowed_stride=allowed_stride, states_stride=states_stride, allowed_rows=allowed_rows)
+        self._point(dict(history=history, history_lengths=history_lengths, history_first=history_first, repetition=repetition,
+                         presence=presence, frequency=frequency, bias_offsets=bias_offsets, bias_ids=bias_ids, bias_values=bias_values,
+                         allowed=allowed, allowed_row=allowed_row, states=states))
+        self._graph = graph
+        self.graph = graph.h.value if graph is not None else None
+
+
+class DrawRules(_Rules):
+    """sky_draw_rules."""
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p)]
+
+    def __init__(self, temperature=None, top_k=None, top_p=None, min_p=None):
+        super().__init__()
+        self._point(dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p))
+
+
+class RouteRules(_Rules):
+    """sky_route_rules."""
+    _fields_ = [("k", C.c_uint32), ("groups", C.c_uint32), ("groups_kept", C.c_uint32), ("sigmoid", C.c_int), ("group_top2", C.c_int),
+                ("renormalise", C.c_int), ("scale", C.c_float), ("bias", C.c_void_p)]
+
+    def __init__(self, k, sigmoid=False, bias=None, groups=1, groups_kept=1, group_top2=False, renormalise=True, scale=1.0):
+        super().__init__(k=k, groups=groups, groups_kept=groups_kept, sigmoid=int(sigmoid), group_top2=int(group_top2),
+                         renormalise=int(renormalise), scale=scale)
+        self._point(dict(bias=bias))
+
+
+def logits_adjust(logits, dtype, rows, columns, rules, out, row_stride=0, out_stride=0, stream=None):
+    """sky_logits_adjust: `out` may be `logits`."""
+    _ck(lib().sky_logits_adjust(_addr(logits), dtype, rows, columns, row_stride, rules.ref if rules is not None else None, _addr(out),
+                                out_stride, stream))
+
+
+def logits_draw_workspace(dtype, rows, columns):
+    """Bytes of workspace that logits_draw makes use of."""
+    n = C.c_uint64(0)
+    _ck(lib().sky_logits_draw_workspace(dtype, rows, columns, C.byref(n)))
+    return n.value
+
+
+def logits_draw(logits, dtype, rows, columns, rules, tokens, uniforms=None, seed=0, first_walker=0, step=0, logprobs=None, kept=None,
+                row_stride=0, tokens_stride=0, workspace=None, workspace_bytes=None, stream=None):
+    """sky_logits_draw.  workspace_bytes None: as many as logits_draw_workspace asks for."""
+    if workspace is None:
+        workspace_bytes = 0
+    elif workspace_bytes is None:
+        workspace_bytes = logits_draw_workspace(dtype, rows, columns)
+    _ck(lib().sky_logits_draw(_addr(logits), dtype, rows, columns, row_stride, rules.ref if rules is not None else None, _addr(uniforms),
+                              seed, first_walker, step, _addr(tokens), tokens_stride, _addr(logprobs), _addr(kept), _addr(workspace),
+                              workspace_bytes, stream))
+
+
+def route_topk(logits, dtype, rows, experts, rules, ids, weights, counts=None, row_stride=0, stream=None):
+    """sky_route_topk."""
+    _ck(lib().sky_route_topk(_addr(logits), dtype, rows, experts, row_stride, rules.ref if rules is not None else None, _addr(ids),
+                             _addr(weights), _addr(counts), stream))
+
+
+def route_topk_backward(logits, dtype, rows, experts, rules, ids, dweights, dlogits, row_stride=0, dlogits_stride=0, stream=None):
+    """sky_route_topk_backward."""
+    _ck(lib().sky_route_topk_backward(_addr(logits), dtype, rows, experts, row_stride, rules.ref if rules is not None else None,
+                                      _addr(ids), _addr(dweights), _addr(dlogits), dlogits_stride, stream))

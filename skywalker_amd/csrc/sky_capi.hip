@@ -15,7 +15,7 @@ int fail(int code, const std::string& msg) {
   return code;
 }
 
-static int ensure_device() {
+int ensure_device() {
   static thread_local bool checked = false;
   if (checked) return SKY_OK;
   int n = 0;

@@ -12,6 +12,7 @@ namespace sky {
 // ---------------------------------------------------------------- error plumbing
 void set_error(const std::string& msg);
 int fail(int code, const std::string& msg);
+int ensure_device();  // SKY_ERR_NO_GPU where the process sees none
 
 #define SKY_HIP(expr)                                                                                 \
   do {                                                                                                \
@@ -30,7 +31,7 @@ int fail(int code, const std::string& msg);
 // ---------------------------------------------------------------- Philox4x32-10
 // Counter = (a, b, c, domain), key = 64-bit seed.  Domains separate the streams of
 // the generators and of the samplers so that no two consumers share a counter.
-enum : uint32_t { DOM_RMAT = 1, DOM_WEIGHT = 2, DOM_SEEDS = 3, DOM_WALK = 4, DOM_SAMPLE = 5 };
+enum : uint32_t { DOM_RMAT = 1, DOM_WEIGHT = 2, DOM_SEEDS = 3, DOM_WALK = 4, DOM_SAMPLE = 5, DOM_LOGITS = 6 };
 
 struct u32x4 {
   uint32_t x, y, z, w;

@@ -1,0 +1,280 @@
+// Logits made ready for a draw (sky_logits_adjust).  For row r and column t, in fp32, rounded to the type once:
+//   y = x                                      seen(t): t is in the row's history, n(t): how often from history_first on
+//   y = x > 0 ? x / rep : x * rep              if seen(t)
+//   y = y - (presence + frequency * n(t))      if n(t) > 0
+//   y = y + bias(t)
+//   y = -inf                                   if a mask or the graph's row does not allow t
+// One pass: every logit is read once and written once, by the same thread, so that a call may work in place.  A workgroup has a
+// tile of a row, 16 columns a thread, and turns the sparse parts (history, biases, neighbours) into arrays over the tile's
+// columns in LDS: counts by integer atomics, whose order does not matter, biases by the thread that meets the first of
+// equal ids.  All of a row's tiles read its whole history, from L2.
+#include "sky_graph.h"
+#include "sky_scores.h"
+
+namespace sky {
+namespace {
+
+constexpr uint32_t COLS = 16;                // columns of a thread
+constexpr uint32_t SEEN = 0x80000000u;       // in the history, before history_first
+constexpr uint32_t BIAS_SEARCH_MIN = 2048u;  // from so many biases on a tile looks for its own by bisection (two chains of some 12 loads)
+
+struct AdjustArgs {
+  const void* logits;
+  void* out;
+  uint64_t stride, out_stride;
+  uint32_t columns, tiles;
+  sky_logits_rules r;
+  const uint32_t* xadj;
+  const uint32_t* adjncy;
+  uint32_t V;
+};
+
+__device__ __forceinline__ uint32_t lower_bound(const uint32_t* a, uint32_t lo, uint32_t hi, uint32_t key) {
+  while (lo < hi) {
+    const uint32_t m = lo + (hi - lo) / 2;
+    if (a[m] < key)
+      lo = m + 1;
+    else
+      hi = m;
+  }
+  return lo;
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void adjust_kernel(AdjustArgs a) {
+  constexpr int N = Piece<T>::N, NV = COLS / N;
+  extern __shared__ uint32_t lds[];
+  const uint32_t threads = blockDim.x, tid = threadIdx.x, tile = COLS * threads;
+  const uint32_t row = blockIdx.x / a.tiles, t = blockIdx.x % a.tiles;
+  const T* const x = (const T*)a.logits + row * a.stride;
+  T* const y = (T*)a.out + row * a.out_stride;
+  // tiles begin where stores are aligned
+  const int phase = (int)((uintptr_t)y / sizeof(T) % N), first = (int)(t * tile) - phase, columns = (int)a.columns;
+  if (first >= columns) return;
+  const uint32_t c0 = (uint32_t)first;  // may wrap: column - c0 is the place in the tile all the same
+  const bool history = a.r.history != nullptr, biased = a.r.bias_ids != nullptr, graph = a.xadj != nullptr;
+  uint32_t mask_row = SKY_INVALID;  // of the bit masks
+  bool none = false;                // nothing of the row is allowed
+  if (a.r.allowed) {
+    mask_row = a.r.allowed_row ? a.r.allowed_row[row] : a.r.allowed_rows == 1 ? 0u : row;
+    none = mask_row != SKY_INVALID && mask_row >= a.r.allowed_rows;
+  }
+  const bool masked = mask_row != SKY_INVALID && !none;
+  const bool whole_tile = first >= 0 && first + (int)tile <= columns;
+
+  Piece<T> v[NV];
+  auto column = [&](int i) { return first + (int)((i * threads + tid) * N); };
+  auto load = [&](int i) {
+    const int c = column(i);
+    if (whole_tile || (c >= 0 && c + N <= columns)) {
+      v[i] = load_piece(x + c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (c + e >= 0 && c + e < columns) v[i].e[e] = x[c + e];
+    }
+  };
+  const bool early = !masked && !graph && !none;  // all of the row is needed: its loads run beside the scans below
+  if (early) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load(i);
+  }
+
+  uint32_t* const count = lds;
+  float* const bias = (float*)(lds + (history ? tile : 0u));
+  uint32_t* const can = lds + (history ? tile : 0u) + (biased ? tile : 0u);
+  const uint32_t words = (history ? tile : 0u) + (biased ? tile : 0u) + (graph ? tile / 32 : 0u);
+  if (words && !none) {
+    for (uint32_t i = tid; i < words / 4; i += threads) ((uint4*)lds)[i] = uint4{0, 0, 0, 0};
+    __syncthreads();
+    if (history) {
+      const uint32_t n = a.r.history_lengths ? min(a.r.history_lengths[row], a.r.history_columns) : a.r.history_columns;
+      const uint32_t from = a.r.history_first ? a.r.history_first[row] : 0u;
+      const uint32_t* const h = a.r.history + row * a.r.history_stride;
+      for (uint32_t i = tid; i < n; i += threads) {
+        const uint32_t id = h[i], at = id - c0;
+        if (at < tile && id < a.columns) {
+          if (i >= from)
+            atomicAdd(&count[at], 1u);
+          else
+            atomicOr(&count[at], SEEN);
+        }
+      }
+    }
+    if (biased) {
+      uint32_t lo = min(a.r.bias_offsets[row], a.r.bias_count), hi = min(a.r.bias_offsets[row + 1], a.r.bias_count);
+      const uint32_t begin = lo, end = hi;
+      if (hi > lo && hi - lo > BIAS_SEARCH_MIN) {
+        lo = lower_bound(a.r.bias_ids, lo, hi, (uint32_t)max(first, 0));
+        hi = lower_bound(a.r.bias_ids, lo, hi, (uint32_t)min((int64_t)first + tile, (int64_t)columns));
+      }
+      for (uint32_t i = lo + tid; i < hi; i += threads) {
+        const uint32_t id = a.r.bias_ids[i], at = id - c0;
+        if (at < tile && id < a.columns && (i == begin || a.r.bias_ids[i - 1] != id)) {
+          float sum = a.r.bias_values[i];
+          for (uint32_t j = i + 1; j < end && a.r.bias_ids[j] == id; ++j) sum += a.r.bias_values[j];
+          bias[at] = sum;
+        }
+      }
+    }
+    if (graph) {
+      const uint32_t s = a.r.states[row * a.r.states_stride];
+      if (s < a.V) {
+        const uint32_t hi = a.xadj[s + 1];
+        for (uint32_t i = a.xadj[s] + tid; i < hi; i += threads) {
+          const uint32_t id = a.adjncy[i], at = id - c0;
+          if (at < tile && id < a.columns) atomicOr(&can[at >> 5], 1u << (at & 31));
+        }
+      }
+    }
+    __syncthreads();
+  }
+  const float rep = history && a.r.repetition ? a.r.repetition[row] : 1.0f;
+  const float presence = history && a.r.presence ? a.r.presence[row] : 0.0f;
+  const float frequency = history && a.r.frequency ? a.r.frequency[row] : 0.0f;
+
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = column(i);
+    const uint32_t at = (i * threads + tid) * N;
+    const bool whole = whole_tile || (c >= 0 && c + N <= columns);
+    uint32_t stay = none ? 0u : (1u << N) - 1;
+    if (masked) {
+      const uint32_t* const m = a.r.allowed + mask_row * a.r.allowed_stride;
+      if (whole) {
+        const uint64_t lo = m[(uint32_t)c >> 5], hi = m[(uint32_t)(c + N - 1) >> 5];
+        stay &= (uint32_t)((lo | hi << 32) >> (c & 31));
+      } else {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (c + e >= 0 && c + e < columns) bits |= (m[(uint32_t)(c + e) >> 5] >> ((c + e) & 31) & 1u) << e;
+        stay &= bits;
+      }
+    }
+    if (graph && !none) stay &= can[at >> 5] >> (at & 31);  // N divides 32: the piece's bits lie in one word
+    if (!early && stay) load(i);
+    Piece<T> o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      float s = (float)v[i].e[e];
+      if (history) {
+        const uint32_t n = count[at + e];
+        if (n) {
+          s = s > 0.0f ? s / rep : s * rep;
+          if (n & ~SEEN) s -= presence + frequency * (float)(n & ~SEEN);
+        }
+      }
+      if (biased) s += bias[at + e];
+      o.e[e] = (T)(stay >> e & 1u ? s : -__builtin_inff());
+    }
+    if (whole) {
+      store_piece(y + c, o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (c + e >= 0 && c + e < columns) y[c + e] = o.e[e];
+    }
+  }
+}
+
+int check_rules(const sky_logits_rules* r, uint32_t rows, uint32_t columns, AdjustArgs* a) {
+  const char* const who = "sky_logits_adjust";
+  auto arg = [&](const char* what) { return fail(SKY_ERR_ARG, std::string(who) + ": " + what); };
+  a->xadj = a->adjncy = nullptr;
+  a->V = 0;
+  if (!r) {
+    a->r = sky_logits_rules{};
+    return SKY_OK;
+  }
+  a->r = *r;
+  if (r->history) {
+    if (!a->r.history_stride) a->r.history_stride = r->history_columns;
+    if (a->r.history_stride < r->history_columns) return arg("history_stride is smaller than history_columns");
+    if (r->history_columns > 0x7FFFFFFFu) return fail(SKY_ERR_LIMIT, std::string(who) + ": more than 2^31 - 1 ids in a history");
+    if (!r->history_columns) a->r.history = nullptr;
+  } else if (r->history_columns || r->history_lengths || r->history_first || r->repetition || r->presence || r->frequency) {
+    return arg("penalties without a history");
+  }
+  if (r->bias_offsets || r->bias_ids || r->bias_values || r->bias_count) {
+    if (!r->bias_count) {  // every row's list is empty
+      a->r.bias_ids = nullptr;
+    } else if (!r->bias_offsets || !r->bias_ids || !r->bias_values) {
+      return arg("biases need offsets, ids and values");
+    }
+  }
+  if (r->allowed) {
+    const uint64_t words = ((uint64_t)columns + 31) / 32;
+    if (!a->r.allowed_stride) a->r.allowed_stride = words;
+    if (a->r.allowed_stride < words) return arg("allowed_stride is smaller than a row of bits");
+    if (!r->allowed_rows) return arg("allowed without rows");
+    if (!r->allowed_row && r->allowed_rows != 1 && r->allowed_rows < rows) return arg("fewer mask rows than rows, and no allowed_row");
+  } else if (r->allowed_rows || r->allowed_row) {
+    return arg("mask rows without masks");
+  }
+  if (r->graph) {
+    if (!r->states) return arg("a graph needs states");
+    if (!a->r.states_stride) a->r.states_stride = 1;
+  } else if (r->states) {
+    return arg("states without a graph");
+  }
+  const struct {
+    const char* name;
+    const void* p;
+  } words[] = {{"history", r->history},           {"history_lengths", r->history_lengths}, {"history_first", r->history_first},
+               {"repetition", r->repetition},     {"presence", r->presence},               {"frequency", r->frequency},
+               {"bias_offsets", r->bias_offsets}, {"bias_ids", r->bias_ids},               {"bias_values", r->bias_values},
+               {"allowed", r->allowed},           {"allowed_row", r->allowed_row},         {"states", r->states}};
+  for (const auto& w : words) SKY_TRY(check_aligned(who, w.name, w.p, 4));
+  return SKY_OK;
+}
+
+}  // namespace
+}  // namespace sky
+
+using namespace sky;
+
+extern "C" int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, uint32_t columns, uint64_t row_stride,
+                                 const sky_logits_rules* rules, void* out, uint64_t out_stride, void* stream) {
+  AdjustArgs a;
+  SKY_TRY(check_rows("sky_logits_adjust", "logits", logits, dtype, rows, columns, &row_stride));
+  SKY_TRY(check_rows("sky_logits_adjust", "out", out, dtype, rows, columns, &out_stride));
+  if (out == logits && out_stride != row_stride) return fail(SKY_ERR_ARG, "sky_logits_adjust: in place with another stride");
+  SKY_TRY(check_rules(rules, rows, columns, &a));
+  if (!rows || !columns) return SKY_OK;
+  SKY_TRY(ensure_device());
+  if (a.r.graph) {
+    int dev = 0;
+    SKY_HIP(hipGetDevice(&dev));
+    if (dev != a.r.graph->device)
+      return fail(SKY_ERR_STATE, "sky_logits_adjust: the graph lives on device " + std::to_string(a.r.graph->device) +
+                                     ", the current device is " + std::to_string(dev));
+    a.xadj = a.r.graph->xadj;
+    a.adjncy = a.r.graph->adjncy;
+    a.V = a.r.graph->V;
+  }
+  a.logits = logits;
+  a.out = out;
+  a.stride = row_stride;
+  a.out_stride = out_stride;
+  a.columns = columns;
+  // counts and biases take 8 bytes of LDS a column: half the tile keeps several workgroups on a CU
+  const uint32_t most = a.r.history && a.r.bias_ids ? 256 : 512;
+  uint32_t threads = 64;
+  while (threads < most && threads * COLS < columns) threads *= 2;
+  const uint32_t tile = threads * COLS;
+  const size_t size = dtype_size(dtype);
+  const bool aligned = ((uintptr_t)out | out_stride * size) % 16 == 0;
+  a.tiles = (uint32_t)(((uint64_t)columns + (aligned ? 0 : 16 / size - 1) + tile - 1) / tile);
+  if ((uint64_t)a.tiles * rows > 0x7FFFFFFFull) return fail(SKY_ERR_LIMIT, "sky_logits_adjust: too many tiles");
+  const size_t lds = ((a.r.history ? tile : 0u) + (a.r.bias_ids ? tile : 0u) + (a.xadj ? tile / 32 : 0u)) * 4;
+  const dim3 grid(a.tiles * rows), block(threads);
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == SKY_F32)
+    hipLaunchKernelGGL(adjust_kernel<float>, grid, block, lds, st, a);
+  else if (dtype == SKY_F16)
+    hipLaunchKernelGGL(adjust_kernel<_Float16>, grid, block, lds, st, a);
+  else
+    hipLaunchKernelGGL(adjust_kernel<__bf16>, grid, block, lds, st, a);
+  return check_launch();
+}
