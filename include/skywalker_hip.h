@@ -288,6 +288,7 @@ int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, uint32_t col
  * tokens[r * tokens_stride] (stride 0: 1) receives it, so that a column of paths can take it, SKY_INVALID where a row has
  * nothing to draw; logprobs[r] (may be NULL) the logarithm of its probability among what stays (-inf for such a row), kept[r] (may
  * be NULL) how many stay.
+ * At most 2^26 columns (SKY_ERR_LIMIT).
  * workspace: memory of the size that sky_logits_draw_workspace gives, aligned to 16 bytes, of which two calls that may run at the same
  * time have one each (a captured graph keeps its own); NULL: every row is drawn from by one workgroup, the same ids, later where
  * there are few rows. */
