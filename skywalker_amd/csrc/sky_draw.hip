@@ -28,7 +28,7 @@ constexpr uint32_t BINS = 2048;      // two per thread
 constexpr uint32_t CAP = 2048;       // entries of a list
 constexpr double NO_MASS = 40.0;     // weights below e^-40 are 0 in units of 2^-S, S <= 50
 constexpr uint32_t SMALL_K = 512;    // of the 1024 threads' largest entries: some 710 entries are as large as the 512th of them
-constexpr uint32_t VALUES = 65536, CHUNK = 64, CHUNKS = VALUES / CHUNK;  // of 16-bit logits; a wavefront takes a chunk
+constexpr uint32_t VALUES = 65536, CHUNK = 256, CHUNKS = VALUES / CHUNK;  // of 16-bit logits; a wavefront takes a chunk, four values a lane
 constexpr int PIECES = 16, AHEAD = 8;  // pieces of 16 bytes that a thread tells apart, and that it has under way at a time
 constexpr uint32_t HITS = THREADS;   // pieces that are read a second time one by one; more: the whole row is
 constexpr uint32_t MAX_COLUMNS = 1u << 26;  // a thread counts its elements in 16 bits
@@ -136,81 +136,93 @@ struct Row {
 };
 
 // ---------------------------------------------------------------- values as places
-// The place of a value: a whole number that ascends with it, turned so that what is not there (NaN, -inf) comes first.  +inf is the
-// largest finite number and -0 is 0.
+// The place of a value: the whole number that its bits, those of negative numbers turned over, make: it ascends with the value.  The
+// place of what is not there (NaN, -inf) is 0, that of +inf the largest finite number's, that of -0 that of 0.
 template <typename T>
 struct Places;
 template <>
 struct Places<float> {
-  static constexpr uint32_t NOTHING = 0xFFFFFEu, TURN = 0x7FFFFFu, TOP_BIT = 0x80000000u;  // up to NOTHING: not there
-  static __device__ __forceinline__ float value(uint32_t q) { return key_score(q - TURN); }
+  static constexpr uint32_t ALL = 0xFFFFFFFFu, SIGN = 0x80000000u, INF = 0x7F800000u, LOWEST = 0x00800000u, LARGEST = 0xFF7FFFFFu;
+  static __device__ __forceinline__ float value(uint32_t q) { return key_score(q); }
 };
 template <>
 struct Places<_Float16> {
-  static constexpr uint32_t NOTHING = 0x7FEu, LOWEST = 0x7FFu, TURN = 0x3FFu, TOP_BIT = 0x8000u;
-  static __device__ __forceinline__ float value(uint32_t q) {
-    const uint32_t k = q - TURN;
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)(k ^ (k & 0x8000u ? 0x8000u : 0xFFFFu)));
-  }
+  static constexpr uint32_t ALL = 0xFFFFu, SIGN = 0x8000u, INF = 0x7C00u, LOWEST = 0x0400u, LARGEST = 0xFBFFu;
+  static __device__ __forceinline__ float value(uint32_t q) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(q ^ (q & SIGN ? SIGN : ALL))); }
 };
 template <>
 struct Places<__bf16> {
-  static constexpr uint32_t NOTHING = 0xFEu, LOWEST = 0xFFu, TURN = 0x7Fu, TOP_BIT = 0x8000u;
-  static __device__ __forceinline__ float value(uint32_t q) {
-    const uint32_t k = q - TURN;
-    return __uint_as_float(((k ^ (k & 0x8000u ? 0x8000u : 0xFFFFu)) & 0xFFFFu) << 16);
-  }
+  static constexpr uint32_t ALL = 0xFFFFu, SIGN = 0x8000u, INF = 0x7F80u, LOWEST = 0x0080u, LARGEST = 0xFF7Fu;
+  static __device__ __forceinline__ float value(uint32_t q) { return __uint_as_float((q ^ (q & SIGN ? SIGN : ALL)) << 16); }
 };
+// The place of one element from its bits.
+template <typename T>
+__device__ __forceinline__ uint32_t place_of_bits(uint32_t b) {
+  using P = Places<T>;
+  const uint32_t size = b & (P::ALL ^ P::SIGN);
+  if (size > P::INF || b == (P::SIGN | P::INF)) return 0;
+  if (size == P::INF) return P::LARGEST;
+  if (!size) return P::SIGN;
+  return b ^ (b & P::SIGN ? P::ALL : P::SIGN);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t place_of(T x) {
+  if constexpr (sizeof(T) == 4)
+    return place_of_bits<T>(__float_as_uint(x));
+  else
+    return place_of_bits<T>(__builtin_bit_cast(uint16_t, x));
+}
+// Words of a row (one 32-bit or two 16-bit elements): bits turned into raw places, which differ from places for what is not finite and
+// for -0 (whose raw place is one less than that of 0).  Two instructions a word; what else a row may hold is looked at piece by piece.
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
-
-// A word of a row (one 32-bit or two 16-bit elements) as places.
 template <typename T>
-__device__ __forceinline__ uint32_t word_places(uint32_t w) {
+__device__ __forceinline__ uint32_t raw_places(uint32_t w) {
   if constexpr (sizeof(T) == 4) {
-    const uint32_t b = __float_as_uint(__uint_as_float(w) + 0.0f);
-    return min((b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) + Places<T>::TURN, 0xFFFFFFFEu);
+    return w ^ ((uint32_t)((int32_t)w >> 31) | 0x80000000u);
   } else {
-    u16x2 v = __builtin_bit_cast(u16x2, w);
-    v &= (u16x2)(-__builtin_elementwise_min(v & (uint16_t)0x7FFF, u16x2{1, 1}));  // -0 is 0
-    const u16x2 sign = __builtin_bit_cast(u16x2, __builtin_bit_cast(i16x2, v) >> (int16_t)15);
-    v = (v ^ (sign | (uint16_t)0x8000)) + (uint16_t)Places<T>::TURN;
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(v, u16x2{0xFFFE, 0xFFFE}));
+    const uint32_t sign = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, w) >> (int16_t)15);
+    return w ^ (sign | 0x80008000u);
   }
 }
-// The larger of two words' places, by element; the largest of a word.
 template <typename T>
 __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b) {
-  if constexpr (sizeof(T) == 4) return max(a, b);
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+  if constexpr (sizeof(T) == 4)
+    return max(a, b);
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 template <typename T>
-__device__ __forceinline__ uint32_t word_most(uint32_t w) {
-  if constexpr (sizeof(T) == 4) return w;
-  return max(w & 0xFFFFu, w >> 16);
-}
-// How many elements of a word lie above a place: added by element, to be taken apart by word_sum (up to 65,535 each).
-template <typename T>
-__device__ __forceinline__ uint32_t word_above(uint32_t w, uint32_t place) {
-  if constexpr (sizeof(T) == 4) return w > place;
-  const u16x2 over = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, w), u16x2{(uint16_t)place, (uint16_t)place});
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(over, u16x2{1, 1}));
+__device__ __forceinline__ uint32_t word_min(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4)
+    return min(a, b);
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 template <typename T>
-__device__ __forceinline__ uint32_t word_sum(uint32_t w) {
-  if constexpr (sizeof(T) == 4) return w;
-  return (w & 0xFFFFu) + (w >> 16);
+__device__ __forceinline__ uint32_t piece_max(uint4 w) {
+  const uint32_t m = word_max<T>(word_max<T>(w.x, w.y), word_max<T>(w.z, w.w));
+  return sizeof(T) == 4 ? m : max(m & 0xFFFFu, m >> 16);
 }
-// f(place, column) for the elements of a piece that begins at column c, in a loop: pieces that are looked at one by one are few.
+template <typename T>
+__device__ __forceinline__ uint32_t piece_min(uint4 w) {
+  const uint32_t m = word_min<T>(word_min<T>(w.x, w.y), word_min<T>(w.z, w.w));
+  return sizeof(T) == 4 ? m : min(m & 0xFFFFu, m >> 16);
+}
+template <typename T>
+__device__ __forceinline__ uint4 raw_places(uint4 w) {
+  return uint4{raw_places<T>(w.x), raw_places<T>(w.y), raw_places<T>(w.z), raw_places<T>(w.w)};
+}
+// f(place, column) for the elements of a piece of bits that begins at column c, in a loop: pieces that are looked at one by one are few.
 template <typename T, typename F>
 __device__ __forceinline__ void each(uint4 w, uint32_t c, F f) {
 #pragma unroll 1
   for (uint32_t e = 0; e < Piece<T>::N; ++e) {
     if constexpr (sizeof(T) == 4) {
-      f(w.x, c + e);
+      f(place_of_bits<T>(w.x), c + e);
       w = uint4{w.y, w.z, w.w, 0};
     } else {
-      f(w.x & 0xFFFFu, c + e);
+      f(place_of_bits<T>(w.x & 0xFFFFu), c + e);
       w = uint4{__builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16), __builtin_amdgcn_alignbit(w.w, w.z, 16), w.w >> 16};
     }
   }
@@ -220,17 +232,6 @@ __device__ __forceinline__ uint4 load_words(const T* p) {
   uint4 w;
   __builtin_memcpy(&w, p, 16);
   return w;
-}
-template <typename T>
-__device__ __forceinline__ uint4 places_of(uint4 w) {
-  return uint4{word_places<T>(w.x), word_places<T>(w.y), word_places<T>(w.z), word_places<T>(w.w)};
-}
-template <typename T>
-__device__ __forceinline__ uint32_t element_place(const T* p) {
-  if constexpr (sizeof(T) == 4)
-    return word_places<T>(__float_as_uint(*p));
-  else
-    return word_places<T>((uint32_t)__builtin_bit_cast(uint16_t, *p)) & 0xFFFFu;
 }
 
 // ---------------------------------------------------------------- lists
@@ -390,14 +391,13 @@ __global__ __launch_bounds__(SHORT_THREADS) void draw_short_kernel(DrawArgs a) {
   if (tid == 0) s.n = 0;
   __syncthreads();
   auto put = [&](uint32_t q, uint32_t c) {
-    if (q > P::NOTHING) {
+    if (q) {
       const uint32_t at = atomicAdd(&s.n, 1u);
       if (at < CAP) s.list[at] = listed(P::value(q), c);
     }
   };
   auto piece = [&](uint4 w, uint32_t c) {
-    w = places_of<T>(w);
-    if (word_most<T>(word_max<T>(word_max<T>(w.x, w.y), word_max<T>(w.z, w.w))) > P::NOTHING) each<T>(w, c, put);
+    if (piece_max<T>(raw_places<T>(w)) >= P::LOWEST) each<T>(w, c, put);
   };
   uint32_t c0 = 0;
   if (SPARSE) {
@@ -419,7 +419,7 @@ __global__ __launch_bounds__(SHORT_THREADS) void draw_short_kernel(DrawArgs a) {
     for (uint32_t i = 0; i < LOADS; ++i) piece(w[i], c0 + i * STEP + tid * N);
   }
   for (uint32_t c = c0 + tid * N; c < whole; c += STEP) piece(load_words(x + c), c);
-  if (whole + tid < columns) put(element_place(x + whole + tid), whole + tid);
+  if (whole + tid < columns) put(place_of(x[whole + tid]), whole + tid);
   __syncthreads();
   const uint32_t n = s.n;
   if (SPARSE && n > CAP) {
@@ -450,150 +450,171 @@ struct Shared {
   };
   uint64_t wave[THREADS / 64];
   uint64_t count_before, mass_before;
-  uint32_t most[THREADS], hit[HITS];
+  uint32_t most[THREADS], hit[HITS], room[CAP];
   uint32_t wave_most[THREADS / 64], wave_least[THREADS / 64], wave_there[THREADS / 64], wave_above[THREADS / 64];
   uint32_t hits, place, chunk, found, lo, hi;
 };
 static_assert(sizeof(Shared) <= 160 * 1024, "LDS of a CU");
 
 // A row as the workgroup's threads read it: PIECES each in turns of THREADS * PIECES, and an entry each of those that do
-// not fill a piece.  Kept of it: the largest place of each of a thread's pieces (over all turns).
+// not fill a piece.  Kept of it: the largest raw place of each of a thread's pieces (over all turns).
 template <typename T>
 struct Reader {
-  static constexpr uint32_t N = Piece<T>::N, TURN = THREADS * PIECES * N;
+  static constexpr uint32_t N = Piece<T>::N, STEP = THREADS * N, TURN = STEP * PIECES;
   using P = Places<T>;
   const T* x;
-  uint32_t columns, whole, turns;
+  uint32_t columns, whole;
   uint32_t most[PIECES];
   uint32_t last;  // place of the odd entry, 0: none
 
-  __device__ __forceinline__ Reader(const T* row, uint32_t n) : x(row), columns(n), whole(n / N * N), turns((n + TURN - 1) / TURN), last(0) {}
-  __device__ __forceinline__ uint32_t column(uint32_t turn, uint32_t i, uint32_t thread) const { return turn * TURN + (i * THREADS + thread) * N; }
-  __device__ __forceinline__ uint4 load(uint32_t c) const {
-    constexpr uint32_t gone = sizeof(T) == 4 ? 0xFF800000u : __is_same(T, _Float16) ? 0xFC00FC00u : 0xFF80FF80u;  // -inf
-    return c < whole ? load_words(x + c) : uint4{gone, gone, gone, gone};
-  }
-  // The first reading: f(word of places) for every word.
-  template <typename F>
-  __device__ __forceinline__ void first(F f) {
-    if (whole + threadIdx.x < columns) last = element_place(x + whole + threadIdx.x);
+  __device__ __forceinline__ Reader(const T* row, uint32_t n) : x(row), columns(n), whole(n / N * N), last(0) {}
+  __device__ __forceinline__ uint4 load(uint32_t c) const { return load_words(x + min(c, whole - N)); }  // of a row of a piece and more
+
+  // The first reading.  f(a piece's raw places) for pieces of finite numbers above the lowest; odd(a piece's bits, column) for the others.
+  // Returns the largest place of the thread.
+  template <typename F, typename G>
+  __device__ __forceinline__ uint32_t first(F f, G odd) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) most[i] = 0;
 #pragma unroll 1
-    for (uint32_t turn = 0; turn < turns; ++turn) {
+    for (uint32_t turn = 0; turn < whole; turn += TURN) {
 #pragma unroll
       for (int h = 0; h < PIECES; h += AHEAD) {
+        if (turn + h * STEP >= whole) break;
         uint4 w[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) w[i] = load(column(turn, h + i, threadIdx.x));
+        for (int i = 0; i < AHEAD; ++i) w[i] = load(turn + (h + i) * STEP + threadIdx.x * N);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           __builtin_amdgcn_sched_barrier(0);  // pieces are worked on as they arrive: all at once they would not fit the registers
-          const uint4 p = places_of<T>(w[i]);
-          f(p.x);
-          f(p.y);
-          f(p.z);
-          f(p.w);
-          most[h + i] = max(most[h + i], word_most<T>(word_max<T>(word_max<T>(p.x, p.y), word_max<T>(p.z, p.w))));
+          const uint32_t c = turn + (h + i) * STEP + threadIdx.x * N;
+          if (c < whole) {
+            const uint4 p = raw_places<T>(w[i]);
+            uint32_t m = piece_max<T>(p);
+            if (m <= P::LARGEST && piece_min<T>(p) > P::LOWEST)
+              f(p);
+            else
+              m = odd(w[i], c);
+            most[h + i] = max(most[h + i], m);
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    f(last);  // of 16 bits: its other half is nothing
-  }
-  __device__ __forceinline__ uint32_t largest() const {
-    uint32_t m = last;
+    uint32_t m = 0;
+    if (whole + threadIdx.x < columns) last = place_of(x[whole + threadIdx.x]);
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) m = max(m, most[i]);
-    return m;
+    return max(m == P::SIGN - 1 ? P::SIGN : m, last);  // -0
   }
-  // f(place, column) for the entries from `least` on: pieces that may hold one are read again, one a thread when they are few.
-  // Called by all threads; a barrier is left to the caller.
-  template <typename F>
-  __device__ __forceinline__ void from(Shared& s, uint32_t least, F f) const {
-    auto look = [&](uint4 w, uint32_t c) {
-      w = places_of<T>(w);
-      if (word_most<T>(word_max<T>(word_max<T>(w.x, w.y), word_max<T>(w.z, w.w))) >= least)
-        each<T>(w, c, [&](uint32_t q, uint32_t col) { if (q >= least) f(q, col); });
-    };
+  // f(piece's bits, column) for every piece that `wanted` (of its raw places) says yes to, of those whose largest place may reach `least`.  They
+  // are read again, one a thread when they are few.  Called by all threads; a barrier is left to the caller.
+  template <typename W, typename F>
+  __device__ __forceinline__ void again(Shared& s, uint32_t least, W wanted, F f) const {
+    const uint32_t raw = least == P::SIGN ? P::SIGN - 1 : least;
     __syncthreads();
     if (threadIdx.x == 0) s.hits = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PIECES; ++i)
-      if (most[i] >= least) {
+      if (most[i] >= raw) {
         const uint32_t at = atomicAdd(&s.hits, 1u);
-        if (at < HITS) s.hit[at] = i * THREADS + threadIdx.x;
+        if (at < HITS) s.hit[at] = (i * THREADS + threadIdx.x) * N;
       }
     __syncthreads();
     const uint32_t hits = s.hits;
     if (hits <= HITS) {
-      if (threadIdx.x < hits) {
-        const uint32_t h = s.hit[threadIdx.x];
-        for (uint32_t turn = 0; turn < turns; ++turn) {
-          const uint32_t c = column(turn, h / THREADS, h % THREADS);
-          if (c < whole) look(load_words(x + c), c);
+      if (threadIdx.x < hits)
+        for (uint32_t c = s.hit[threadIdx.x]; c < whole; c += TURN) {
+          const uint4 w = load_words(x + c);
+          if (wanted(raw_places<T>(w))) f(w, c);
         }
-      }
     } else {
 #pragma unroll 1
-      for (uint32_t c = threadIdx.x * N; c < whole; c += 4 * THREADS * N) {
-        uint4 w[4];
+      for (uint32_t c = threadIdx.x * N; c < whole; c += AHEAD * STEP) {
+        uint4 w[AHEAD];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) w[i] = load(c + i * THREADS * N);
+        for (uint32_t i = 0; i < AHEAD; ++i) w[i] = load(c + i * STEP);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) look(w[i], c + i * THREADS * N);
+        for (uint32_t i = 0; i < AHEAD; ++i)
+          if (c + i * STEP < whole && wanted(raw_places<T>(w[i]))) f(w[i], c + i * STEP);
       }
     }
+  }
+  // f(place, column) for the entries from `least` on
+  template <typename F>
+  __device__ __forceinline__ void from(Shared& s, uint32_t least, F f) const {
+    const uint32_t raw = least == P::SIGN ? P::SIGN - 1 : least;
+    again(s, least, [&](uint4 p) { return piece_max<T>(p) >= raw; },
+          [&](uint4 w, uint32_t c) { each<T>(w, c, [&](uint32_t q, uint32_t col) { if (q >= least) f(q, col); }); });
     if (last >= least) f(last, whole + threadIdx.x);
+  }
+  // f(column) for the entries of a place
+  template <typename F>
+  __device__ __forceinline__ void equal(Shared& s, uint32_t place, F f) const {
+    // what is 0 in a word that holds the place's raw bits; two kinds of bits are the place of 0 and that of the largest number
+    const uint32_t other = place == P::SIGN ? P::SIGN - 1 : place == P::LARGEST ? P::LARGEST + 1 : place;
+    const uint32_t a = sizeof(T) == 4 ? place : place | place << 16, b = sizeof(T) == 4 ? other : other | other << 16;
+    again(s, place, [&](uint4 p) {
+      uint32_t m = piece_min<T>(uint4{p.x ^ a, p.y ^ a, p.z ^ a, p.w ^ a});
+      if (a != b) m = min(m, piece_min<T>(uint4{p.x ^ b, p.y ^ b, p.z ^ b, p.w ^ b}));
+      return m == 0;
+    }, [&](uint4 w, uint32_t c) { each<T>(w, c, [&](uint32_t q, uint32_t col) { if (q == place) f(col); }); });
+    if (last == place) f(whole + threadIdx.x);
   }
   // f(value, column) for every entry that is there: later readings of the whole row
   template <typename F>
   __device__ __forceinline__ void all(F f) const {
 #pragma unroll 1
-    for (uint32_t c = threadIdx.x * N; c < whole; c += 4 * THREADS * N) {
+    for (uint32_t c = threadIdx.x * N; c < whole; c += 4 * STEP) {
       uint4 w[4];
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) w[i] = load(c + i * THREADS * N);
+      for (uint32_t i = 0; i < 4; ++i) w[i] = load(c + i * STEP);
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
         __builtin_amdgcn_sched_barrier(0);
-        auto one = [&](uint32_t q, uint32_t col) { if (q > P::NOTHING) f(P::value(q), col); };
-        const uint4 p = places_of<T>(w[i]);
-        if constexpr (sizeof(T) == 4) {
-          one(p.x, c + i * THREADS * N);
-          one(p.y, c + i * THREADS * N + 1);
-          one(p.z, c + i * THREADS * N + 2);
-          one(p.w, c + i * THREADS * N + 3);
-        } else {
-          each<T>(p, c + i * THREADS * N, one);
+        const uint32_t at = c + i * STEP;
+        if (at < whole) {
+          if constexpr (sizeof(T) == 4) {
+            // NaN and -inf pass no test of a value, +inf is the largest number
+            auto one = [&](uint32_t bits, uint32_t col) {
+              const float z = __uint_as_float(bits);
+              f((z > 3.402823466e38f ? 3.402823466e38f : z) + 0.0f, col);  // -0 is 0
+            };
+            one(w[i].x, at);
+            one(w[i].y, at + 1);
+            one(w[i].z, at + 2);
+            one(w[i].w, at + 3);
+          } else {
+            each<T>(w[i], at, [&](uint32_t q, uint32_t col) { if (q) f(P::value(q), col); });
+          }
         }
       }
     }
-    if (last > P::NOTHING) f(P::value(last), whole + threadIdx.x);
+    if (last) f(P::value(last), whole + threadIdx.x);
   }
 };
 
 // The column of entry `tie` among those of value z, by column: as few of them as the list holds are listed, more are counted off.
 template <typename T>
-__device__ uint32_t column_of_tie(const Reader<T>& in, Shared& s, uint32_t* list, uint32_t q, uint32_t tie, uint32_t ties) {
+__device__ __forceinline__ uint32_t column_of_tie(const Reader<T>& in, Shared& s, uint32_t q, uint32_t tie, uint32_t ties) {
   __syncthreads();
   if (threadIdx.x == 0) s.found = SKY_INVALID;
   if (ties <= CAP) {
     if (threadIdx.x == 0) s.place = 0;
-    in.from(s, q, [&](uint32_t v, uint32_t c) { if (v == q) list[atomicAdd(&s.place, 1u)] = c; });
+    in.equal(s, q, [&](uint32_t c) { s.room[atomicAdd(&s.place, 1u)] = c; });
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < ties; i += THREADS) {
       uint32_t below = 0;
-      const uint32_t c = list[i];
-      for (uint32_t j = 0; j < ties; ++j) below += list[j] < c;
+      const uint32_t c = s.room[i];
+      for (uint32_t j = 0; j < ties; ++j) below += s.room[j] < c;
       if (below == tie) s.found = c;
     }
   } else {
     uint64_t seen = 0;
     for (uint32_t base = 0; base < in.columns && seen <= tie; base += THREADS) {
       const uint32_t c = base + threadIdx.x;
-      const uint64_t here = c < in.columns && element_place(in.x + c) == q;
+      const uint64_t here = c < in.columns && place_of(in.x[c]) == q;
       uint64_t total;
       const uint64_t before = seen + block_scan<THREADS>(here, s.wave, &total);
       if (here && before == tie) s.found = c;
@@ -605,27 +626,35 @@ __device__ uint32_t column_of_tie(const Reader<T>& in, Shared& s, uint32_t* list
 }
 
 // ---------------------------------------------------------------- by value
-// One chunk of values, the largest first: lane l has its l-th largest.
-struct Chunk {
-  uint32_t q, count;
-  float z;
-  uint64_t mass;
-};
 __device__ __forceinline__ uint32_t count_of(const Counters& c, uint32_t q) {
   const uint32_t both = c.value[q & 0x7FFFu];
   return q & 0x8000u ? both >> 16 : both & 0xFFFFu;
 }
-template <typename T>
-__device__ __forceinline__ Chunk chunk_of(const Counters& c, uint32_t chunk, const Row& row) {
-  Chunk r;
-  r.q = chunk * CHUNK + (CHUNK - 1) - (threadIdx.x & 63);
-  r.count = count_of(c, r.q);
-  r.z = r.count ? Places<T>::value(r.q) : row.zmax;
-  r.mass = r.count ? r.count * row.units(r.z) : 0;
-  return r;
+// A lane's four values of a chunk, the largest first: lane 0 has the four largest.
+struct Values {
+  uint32_t q;         // place of the largest; the others follow downwards
+  uint32_t count[4];
+  uint64_t mass[4];   // of all entries of the value
+  __device__ __forceinline__ uint32_t counts() const { return count[0] + count[1] + count[2] + count[3]; }
+  __device__ __forceinline__ uint64_t masses() const { return mass[0] + mass[1] + mass[2] + mass[3]; }
+};
+__device__ __forceinline__ bool values_of(const Counters& c, uint32_t chunk, Values* v) {
+  v->q = chunk * CHUNK + (CHUNK - 1) - 4 * (threadIdx.x & 63);
+  uint4 w = *(const uint4*)&c.value[(v->q - 3) & 0x7FFFu];
+  const uint32_t shift = v->q & 0x8000u ? 16 : 0;
+  v->count[0] = w.w >> shift & 0xFFFFu;
+  v->count[1] = w.z >> shift & 0xFFFFu;
+  v->count[2] = w.y >> shift & 0xFFFFu;
+  v->count[3] = w.x >> shift & 0xFFFFu;
+  return __ballot(v->counts() != 0) != 0;
 }
-// The value that holds a unit (RANK: of the count; else of mass), from the sums of chunks before each thread's own (thread t has the
-// t-th chunk from the top).
+template <typename T>
+__device__ __forceinline__ void weigh(const Row& row, Values* v) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v->mass[j] = v->count[j] ? v->count[j] * row.units(Places<T>::value(v->q - j)) : 0;
+}
+// The value that holds a unit (RANK: of the count; else of mass), from the sums of chunks before each thread's own (thread t < CHUNKS has
+// the t-th chunk from the top).
 struct ValuePlace {
   uint32_t q, tie;
   float z;
@@ -633,67 +662,87 @@ struct ValuePlace {
 };
 template <bool RANK, typename T>
 __device__ __forceinline__ ValuePlace locate_value(Shared& s, const Row& row, uint64_t unit, uint64_t count_before, uint64_t mass_before) {
-  const uint32_t mine = CHUNKS - 1 - threadIdx.x;
-  const uint64_t before = RANK ? count_before : mass_before;
-  const uint64_t here = RANK ? (uint64_t)s.counters.chunk_count[mine] : s.counters.chunk_mass[mine];
   __syncthreads();
-  if (before <= unit && unit < before + here) {
-    s.chunk = mine;
-    s.count_before = count_before;
-    s.mass_before = mass_before;
+  if (threadIdx.x < CHUNKS) {
+    const uint32_t mine = CHUNKS - 1 - threadIdx.x;
+    const uint64_t before = RANK ? count_before : mass_before;
+    const uint64_t here = RANK ? (uint64_t)s.counters.chunk_count[mine] : s.counters.chunk_mass[mine];
+    if (before <= unit && unit < before + here) {
+      s.chunk = mine;
+      s.count_before = count_before;
+      s.mass_before = mass_before;
+    }
   }
   __syncthreads();
-  const Chunk k = chunk_of<T>(s.counters, s.chunk, row);
-  const uint64_t counts = s.count_before + group_scan_u64<64>(k.count) - k.count;
-  const uint64_t masses = s.mass_before + group_scan_u64<64>(k.mass) - k.mass;
-  const uint64_t start = RANK ? counts : masses, size = RANK ? (uint64_t)k.count : k.mass;
-  const int lane = (int)__builtin_ctzll(__ballot(start <= unit && unit < start + size) | 1ull << 63);
-  ValuePlace p;
-  p.q = (uint32_t)__shfl((int)k.q, lane, 64);
-  p.z = __shfl(k.z, lane, 64);
-  p.count_before = shfl_u64(counts, lane);
-  p.mass_before = shfl_u64(masses, lane);
-  p.tie = (uint32_t)((unit - (RANK ? p.count_before : p.mass_before)) / (RANK ? 1 : row.units(p.z)));
+  Values v;
+  values_of(s.counters, s.chunk, &v);
+  weigh<T>(row, &v);
+  uint64_t counts = s.count_before + group_scan_u32<64>(v.counts()) - v.counts(), masses = s.mass_before + group_scan_u64<64>(v.masses()) - v.masses();
+  ValuePlace p{0, 0, 0.0f, 0, 0};
+  bool here = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint64_t start = RANK ? counts : masses, size = RANK ? (uint64_t)v.count[j] : v.mass[j];
+    if (start <= unit && unit < start + size) {
+      here = true;
+      p.q = v.q - j;
+      p.count_before = counts;
+      p.mass_before = masses;
+    }
+    counts += v.count[j];
+    masses += v.mass[j];
+  }
+  const int lane = (int)__builtin_ctzll(__ballot(here) | 1ull << 63);
+  p.q = (uint32_t)__shfl((int)p.q, lane, 64);
+  p.count_before = shfl_u64(p.count_before, lane);
+  p.mass_before = shfl_u64(p.mass_before, lane);
+  p.z = Places<T>::value(p.q);
+  p.tie = RANK ? (uint32_t)(unit - p.count_before) : (uint32_t)((unit - p.mass_before) / row.units(p.z));
   return p;
 }
 // The largest place up to `most` whose value fails `passes`, which holds from some place on; what is not there fails.
 template <typename T, typename F>
 __device__ __forceinline__ uint32_t last_failing(uint32_t most, F passes) {
   uint32_t lo = 0;
-  for (uint32_t bit = Places<T>::TOP_BIT; bit; bit >>= 1) {
+  for (uint32_t bit = Places<T>::SIGN; bit; bit >>= 1) {
     const uint32_t q = lo | bit;
-    if (q <= most && (q <= Places<T>::NOTHING || !passes(Places<T>::value(q)))) lo = q;
+    if (q <= most && (q < Places<T>::LOWEST || !passes(Places<T>::value(q)))) lo = q;
   }
   return lo;
 }
 __device__ __forceinline__ void clear_counters(Counters& c) {
   for (uint32_t i = threadIdx.x; i < VALUES / 8; i += THREADS) ((uint4*)c.value)[i] = uint4{0, 0, 0, 0};
 }
-// Every element of a word that is above the lowest value, which masks are made of and which is counted by subtraction.
-template <typename T>
+__device__ __forceinline__ void count_place(Counters& c, uint32_t q) { atomicAdd(&c.value[q & 0x7FFFu], (q >> 15) * 0xFFFFu + 1u); }
 __device__ __forceinline__ void count_word(Counters& c, uint32_t w) {
-  const uint32_t lo = w & 0xFFFFu, hi = w >> 16;
-  if (lo > Places<T>::LOWEST) atomicAdd(&c.value[lo & 0x7FFFu], lo & 0x8000u ? 0x10000u : 1u);
-  if (hi > Places<T>::LOWEST) atomicAdd(&c.value[hi & 0x7FFFu], hi & 0x8000u ? 0x10000u : 1u);
+  count_place(c, w & 0xFFFFu);
+  count_place(c, w >> 16);
 }
 
-// A row that has been counted; false: a counter has run over, or the lowest value weighs something.
+// A row that has been counted, all but entries of the lowest value, which masks are made of: `above` of `there`.  false: a counter
+// has run over, or the lowest value weighs something.
 template <typename T>
 __device__ __forceinline__ bool draw_by_value(const Reader<T>& in, Shared& s, const Row& row, const Settings& o, double u, uint32_t most, uint32_t there,
                                               uint32_t above, Result* result) {
   using P = Places<T>;
   Counters& c = s.counters;
   if (there != above && row.units(P::value(P::LOWEST))) return false;
+  if (threadIdx.x == 0) {  // what was counted as -0 is 0
+    const uint32_t n = c.value[P::SIGN - 1] & 0xFFFFu;
+    c.value[P::SIGN - 1] -= n;
+    c.value[0] += n << 16;
+  }
+  __syncthreads();
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  // a wavefront takes every 16th chunk
-#pragma unroll 4
-  for (uint32_t i = 0; i < CHUNKS / (THREADS / 64); ++i) {
-    const uint32_t chunk = i * (THREADS / 64) + wave, q = chunk * CHUNK + lane, n = count_of(c, q);
+  // a wavefront takes every 16th chunk: those that occur lie together
+  for (uint32_t chunk = wave; chunk < CHUNKS; chunk += THREADS / 64) {
+    Values v;
     uint64_t mass = 0;
     uint32_t count = 0;
-    if (__ballot(n != 0)) {
-      count = group_scan_u32<64>(n);
-      mass = group_scan_u64<64>(n ? n * row.units(P::value(q)) : 0);
+    if (values_of(c, chunk, &v)) {
+      weigh<T>(row, &v);
+      count = group_scan_u32<64>(v.counts());
+      mass = group_scan_u64<64>(v.masses());
     }
     if (lane == 63) {
       c.chunk_count[chunk] = count;
@@ -703,8 +752,9 @@ __device__ __forceinline__ bool draw_by_value(const Reader<T>& in, Shared& s, co
   __syncthreads();
   uint64_t counted, mass;
   const uint32_t mine = CHUNKS - 1 - threadIdx.x;
-  const uint64_t count_before = block_scan<THREADS>(c.chunk_count[mine], s.wave, &counted);
-  const uint64_t mass_before = block_scan<THREADS>(c.chunk_mass[mine], s.wave, &mass);
+  const bool own = threadIdx.x < CHUNKS;
+  const uint64_t count_before = block_scan<THREADS>(own ? c.chunk_count[mine] : 0, s.wave, &counted);
+  const uint64_t mass_before = block_scan<THREADS>(own ? c.chunk_mass[mine] : 0, s.wave, &mass);
   if (counted != above) return false;
   uint32_t count = there;
   if (o.top_k && o.top_k < there) {
@@ -722,23 +772,31 @@ __device__ __forceinline__ bool draw_by_value(const Reader<T>& in, Shared& s, co
   if (o.min_p > 0.0f) {
     const uint32_t least = min(last_failing<T>(most, [&](float z) { return row.weight(z) >= (double)o.min_p; }) + 1, most), chunk = least / CHUNK;
     __syncthreads();
-    if (mine == chunk) {
+    if (own && mine == chunk) {
       s.count_before = count_before;
       s.mass_before = mass_before;
     }
     __syncthreads();
-    const Chunk k = chunk_of<T>(c, chunk, row);
-    const uint64_t in_count = s.count_before + shfl_u64(group_scan_u64<64>(k.q >= least ? k.count : 0), 63);
-    const uint64_t in_mass = s.mass_before + shfl_u64(group_scan_u64<64>(k.q >= least ? k.mass : 0), 63);
-    if (least > P::LOWEST && in_count < count) {
-      count = (uint32_t)in_count;
-      mass = in_mass;
+    Values v;
+    values_of(c, chunk, &v);
+    weigh<T>(row, &v);
+    uint32_t in_count = 0;
+    uint64_t in_mass = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (v.q - j >= least) {
+        in_count += v.count[j];
+        in_mass += v.mass[j];
+      }
+    const uint64_t all_count = s.count_before + (uint32_t)__shfl((int)group_scan_u32<64>(in_count), 63, 64);
+    const uint64_t all_mass = s.mass_before + shfl_u64(group_scan_u64<64>(in_mass), 63);
+    if (least > P::LOWEST && all_count < count) {
+      count = (uint32_t)all_count;
+      mass = all_mass;
     }
   }
   const ValuePlace p = locate_value<false, T>(s, row, Row::drawn(u, mass), count_before, mass_before);
-  const uint32_t ties = count_of(c, p.q);
-  static_assert(sizeof(c.chunk_mass) == CAP * 4, "the sums of chunks, which nobody reads any more, make room for the list");
-  *result = Result{column_of_tie(in, s, (uint32_t*)c.chunk_mass, p.q, p.tie, ties), count, row.log_share(p.z, mass)};
+  *result = Result{column_of_tie(in, s, p.q, p.tie, count_of(c, p.q)), count, row.log_share(p.z, mass)};
   return true;
 }
 
@@ -747,10 +805,14 @@ __device__ __forceinline__ bool draw_by_value(const Reader<T>& in, Shared& s, co
 // that is hi).
 struct Bins {
   double hi, scale;
-  float top, low;
-  __device__ __forceinline__ Bins(float h, float l) : hi(h), scale(h > l ? (double)(BINS - 1) / ((double)h - (double)l) : 0.0), top(h), low(l) {}
+  float top, low, narrow;  // narrow: the scale in fp32, 0 where that might not tell lo and hi apart (very wide and very narrow intervals)
+  __device__ __forceinline__ Bins(float h, float l) : hi(h), scale(h > l ? (double)(BINS - 1) / ((double)h - (double)l) : 0.0), top(h), low(l) {
+    narrow = scale > 1e-30 && scale < 1e30 ? (float)scale : 0.0f;
+  }
   __device__ __forceinline__ bool has(float z) const { return z <= top && z >= low; }
-  __device__ __forceinline__ uint32_t of(float z) const { return min((uint32_t)((hi - (double)z) * scale), BINS - 1); }
+  __device__ __forceinline__ uint32_t of(float z) const {
+    return min(narrow != 0.0f ? (uint32_t)((top - z) * narrow) : (uint32_t)((hi - (double)z) * scale), BINS - 1);
+  }
 };
 // Where an answer lies: the value, how many entries of it come before, how many there are, the column (SKY_INVALID: to be looked
 // for), and what all entries before the value amount to (units of mass or entries).
@@ -898,7 +960,7 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, c
   }
   if (o.min_p > 0.0f && (row.weight(end) < (double)o.min_p || (cut_off && !(o.top_p < 1.0f)))) {
     const uint32_t least = min(last_failing<T>(most, [&](float z) { return row.weight(z) >= (double)o.min_p; }) + 1, most);
-    const float z_least = Places<T>::value(max(least, Places<T>::NOTHING + 1));
+    const float z_least = Places<T>::value(max(least, Places<T>::LOWEST));
     uint64_t weighs = 0, many = 0, all, all_many;
     in.all([&](float z, uint32_t) {
       if (z >= z_least) {
@@ -916,8 +978,7 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, c
   const Place p = locate<false>(in, s, row, bins, f, low, excess, Row::drawn(u, mass));
   Result r{p.column, count, row.log_share(p.z, mass)};
   if (r.token == SKY_INVALID) {
-    const T exact = (T)p.z;
-    r.token = column_of_tie(in, s, (uint32_t*)s.bin, element_place(&exact), p.tie, p.ties);
+    r.token = column_of_tie(in, s, place_of((T)p.z), p.tie, p.ties);
   }
   return r;
 }
@@ -927,28 +988,57 @@ template <typename T>
 __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared& s, const Settings& o, double u) {
   using P = Places<T>;
   constexpr bool BY_VALUE = sizeof(T) == 2;
-  const bool greedy = o.greedy(), small_k = o.top_k && o.top_k <= SMALL_K, only_min_p = o.min_p > 0.0f && !(o.top_p < 1.0f);
-  const bool few = greedy || small_k || (only_min_p && !BY_VALUE);  // few entries can stay
+  const bool greedy = o.greedy(), small_k = o.top_k && o.top_k <= SMALL_K, only_min_p = !BY_VALUE && o.min_p > 0.0f && !(o.top_p < 1.0f);
+  const bool few = greedy || small_k || only_min_p;  // few entries can stay
   Reader<T> in(x, columns);
-  uint32_t there_w = 0, above_w = 0, least = 0xFFFFFFFFu;
+  uint32_t most, there = 0, above = 0, least = 0xFFFFFFFFu;  // above: the lowest value
   if constexpr (BY_VALUE) {
-    auto take = [&](uint32_t w) {
-      there_w += word_above<T>(w, P::NOTHING);
-      above_w += word_above<T>(w, P::LOWEST);
+    auto odd = [&](uint4 w, uint32_t c) {
+      uint32_t m = 0;
+      each<T>(w, c, [&](uint32_t q, uint32_t) {
+        m = max(m, q);
+        there += q != 0;
+        above += q > P::LOWEST;
+        if (!few && q > P::LOWEST) count_place(s.counters, q);
+      });
+      return m;
     };
-    if (!few) clear_counters(s.counters);
-    __syncthreads();
-    in.first([&](uint32_t w) {
-      take(w);
-      if (!few) count_word<T>(s.counters, w);
-    });
+    auto regular = [&](uint32_t n) {
+      there += n;
+      above += n;
+    };
+    if (few) {
+      most = in.first([&](uint4) { regular(Piece<T>::N); }, odd);
+    } else {
+      clear_counters(s.counters);
+      __syncthreads();
+      most = in.first([&](uint4 p) {
+        regular(Piece<T>::N);
+        count_word(s.counters, p.x);
+        count_word(s.counters, p.y);
+        count_word(s.counters, p.z);
+        count_word(s.counters, p.w);
+      }, odd);
+      if (in.last > P::LOWEST) count_place(s.counters, in.last);
+    }
+    there += in.last != 0;
+    above += in.last > P::LOWEST;
   } else {
-    in.first([&](uint32_t w) {
-      there_w += word_above<T>(w, P::NOTHING);
-      least = w > P::NOTHING ? min(least, w) : least;
+    most = in.first([&](uint4 p) {
+      there += Piece<T>::N;
+      least = min(least, piece_min<T>(p));
+    }, [&](uint4 w, uint32_t c) {
+      uint32_t m = 0;
+      each<T>(w, c, [&](uint32_t q, uint32_t) {
+        m = max(m, q);
+        there += q != 0;
+        least = q ? min(least, q) : least;
+      });
+      return m;
     });
+    there += in.last != 0;
+    least = in.last ? min(least, in.last) : least;
   }
-  uint32_t most = in.largest(), there = word_sum<T>(there_w), above = word_sum<T>(above_w);
   {
     const uint32_t w = threadIdx.x >> 6;
     s.most[threadIdx.x] = most;
@@ -972,31 +1062,53 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared&
   if (!there) return nothing_to_draw();
   if (greedy) {
     if (threadIdx.x == 0) s.place = SKY_INVALID;
-    in.from(s, most, [&](uint32_t, uint32_t c) { atomicMin(&s.place, c); });
+    in.equal(s, most, [&](uint32_t c) { atomicMin(&s.place, c); });
     __syncthreads();
     return Result{s.place, 1, 0.0};
   }
   const Row row(o.temperature, P::value(most), fraction_bits(columns));
   if (few || there <= CAP) {
-    uint32_t from = P::NOTHING + 1;  // places from here on are listed
+    uint32_t from = 1;  // places from here on are listed
     if (there > CAP && small_k) {
-      // the top_k-th largest of the threads' largest: at least top_k entries are as large
+      // A place that at least top_k of the threads' largest reach, and few more: at least top_k entries reach it.  Up to 128 the
+      // largest of four threads do.
       if (threadIdx.x < 64) {
-        uint32_t v[THREADS / 64], lo = 0;
+        uint32_t v[THREADS / 64], lo = 0, hi = most;  // top_k or more reach lo, fewer reach more than hi
+        const bool quads = o.top_k <= THREADS / 8;
 #pragma unroll
         for (int i = 0; i < THREADS / 64; ++i) v[i] = s.most[64 * i + threadIdx.x];
-        for (uint32_t bit = P::TOP_BIT; bit; bit >>= 1) {
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; i += 4)
+          if (quads) v[i / 4] = max(max(v[i], v[i + 1]), max(v[i + 2], v[i + 3]));
+        auto reach = [&](uint32_t place) {
           uint32_t n = 0;
 #pragma unroll
-          for (int i = 0; i < THREADS / 64; ++i) n += (uint32_t)__builtin_popcountll(__ballot(v[i] >= (lo | bit)));
-          if (n >= o.top_k) lo |= bit;
+          for (int i = 0; i < 4; ++i) n += (uint32_t)__builtin_popcountll(__ballot(v[i] >= place));
+          if (!quads)
+#pragma unroll
+            for (int i = 4; i < THREADS / 64; ++i) n += (uint32_t)__builtin_popcountll(__ballot(v[i] >= place));
+          return n;
+        };
+        uint32_t smallest = v[0];
+#pragma unroll
+        for (int i = 1; i < THREADS / 64; ++i)
+          if (i < 4 || !quads) smallest = min(smallest, v[i]);
+        lo = wave_min_u32(smallest);  // all of them reach it
+        while (lo < hi) {
+          const uint32_t mid = lo + (hi - lo + 1) / 2, n = reach(mid);
+          if (n >= o.top_k) {
+            lo = mid;
+            if (n <= o.top_k + 16) break;
+          } else {
+            hi = mid - 1;
+          }
         }
         if (threadIdx.x == 0) s.place = lo;
       }
       __syncthreads();
       from = max(from, s.place);
     }
-    if (there > CAP && only_min_p && !BY_VALUE) {
+    if (there > CAP && only_min_p) {
       // the smallest value that may weigh min_p, with a margin for the logarithm
       const double z = (double)row.zmax + row.t * (log((double)o.min_p) - 1e-6) - 1e-6 * fabs((double)row.zmax);
       from = max(from, min(last_failing<T>(most, [&](float v) { return (double)v >= z; }) + 1, most));
@@ -1016,7 +1128,7 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared&
     Result r;
     if (!few && draw_by_value(in, s, row, o, u, most, there, above, &r)) return r;
     __syncthreads();
-    least = P::NOTHING + 1;
+    least = P::LOWEST;
   }
   return draw_by_bins(in, s, row, o, u, most, P::value(least), there);
 }
