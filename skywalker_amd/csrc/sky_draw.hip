@@ -29,7 +29,7 @@ constexpr uint32_t CAP = 2048;       // entries of a list
 constexpr double NO_MASS = 40.0;     // weights below e^-40 are 0 in units of 2^-S, S <= 50
 constexpr uint32_t SMALL_K = 512;    // of the 1024 threads' largest entries: some 710 entries are as large as the 512th of them
 constexpr uint32_t VALUES = 65536, CHUNK = 256, CHUNKS = VALUES / CHUNK;  // of 16-bit logits; a wavefront takes a chunk, four values a lane
-constexpr int PIECES = 16, AHEAD = 8;  // pieces of 16 bytes that a thread tells apart, and that it has under way at a time
+constexpr int PIECES = 16, AHEAD = 4;  // pieces of 16 bytes that a thread tells apart, and of a load that runs while as many are worked on
 constexpr uint32_t HITS = THREADS;   // pieces that are read a second time one by one; more: the whole row is
 constexpr uint32_t MAX_COLUMNS = 1u << 26;  // a thread counts its elements in 16 bits
 constexpr uint32_t NOT_DRAWN = 0xFFFFFFFEu;  // token of a row that draw_short_kernel leaves to draw_kernel
@@ -122,7 +122,15 @@ struct Row {
   __device__ __forceinline__ double weight(float z) const { return exp(((double)z - (double)zmax) / t); }
   __device__ __forceinline__ uint64_t units(float z) const {
     const double x = ((double)z - (double)zmax) * per;
-    return x >= -60.0 ? power_units(x, S) : 0;
+    const uint64_t n = power_units(fmax(x, -60.0), S);
+    return x >= -60.0 ? n : 0;
+  }
+  // rest / each, which is below 2^27
+  static __device__ __forceinline__ uint32_t quotient(uint64_t rest, uint64_t each) {
+    uint32_t q = (uint32_t)((double)rest / (double)each);  // off by one at most: both are rounded to 53 bits
+    if ((uint64_t)q * each > rest) --q;
+    if (rest - (uint64_t)q * each >= each) ++q;
+    return q;
   }
   // the logarithm of z's share of `mass` units
   __device__ __forceinline__ double log_share(float z, uint64_t mass) const {
@@ -267,9 +275,25 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* waves, uint
   return before + inclusive - v;
 }
 
-// list[0..m) into the order: a bitonic network over the next power of two, at least 64.
+// list[0..m) into the order.  Up to an entry a thread: every entry's rank is counted (no barrier between the steps); longer lists
+// by a bitonic network over the next power of two.  (Lists of 64: 1.2 us less than by the network.)
 template <int BT>
 __device__ __forceinline__ void sort_list(uint64_t* list, uint32_t m) {
+  if (m <= BT / 2) {
+    const uint64_t mine = threadIdx.x < m ? list[threadIdx.x] : LIST_END;
+    uint32_t rank = 0;
+    if (threadIdx.x < m) {
+      uint32_t i = 0;
+      for (; i + 8 <= m; i += 8)
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) rank += list[i + j] < mine;
+      for (; i < m; ++i) rank += list[i] < mine;
+    }
+    __syncthreads();
+    if (threadIdx.x < m) list[rank] = mine;
+    __syncthreads();
+    return;
+  }
   uint32_t size = 64;
   while (size < m) size *= 2;
   for (uint32_t i = m + threadIdx.x; i < size; i += BT) list[i] = LIST_END;
@@ -288,16 +312,18 @@ __device__ __forceinline__ void sort_list(uint64_t* list, uint32_t m) {
     }
 }
 
-// Everything about a row whose entries, or as many of them as can matter, are one to a lane of this wavefront, in any order, n of them
-// (lanes from n on: LIST_END).
-__device__ __forceinline__ Result draw_wave(uint64_t e, uint32_t n, const Settings& o, double u) {
+// Everything about a row whose entries, or as many of them as can matter, are list[0..n), n <= 64, in any order: by one wavefront.
+__device__ __forceinline__ Result draw_wave(uint64_t* list, uint32_t n, const Settings& o, double u) {
   const uint32_t lane = threadIdx.x & 63;
-  for (uint32_t k = 2; k < 2 * n; k *= 2)
-    for (uint32_t j = k / 2; j; j /= 2) {
-      const uint64_t other = shfl_xor_u64(e, (int)j);
-      const bool low = (lane & j) == 0, up = (lane & k) == 0;
-      e = (other < e) == (low == up) ? other : e;
-    }
+  uint64_t e = lane < n ? list[lane] : LIST_END;
+  uint32_t rank = 0;
+  for (uint32_t i = 0; i < n; i += 4)
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) rank += i + j < n && list[i + j] < e;
+  __builtin_amdgcn_wave_barrier();
+  if (lane < n) list[rank] = e;
+  __builtin_amdgcn_wave_barrier();
+  e = lane < n ? list[lane] : LIST_END;
   const Row row(o.temperature, listed_score(shfl_u64(e, 0)), 50);
   const uint32_t k = o.top_k && o.top_k < n ? o.top_k : n;
   const float z = lane < k ? listed_score(e) : row.zmax;
@@ -364,7 +390,7 @@ __device__ __forceinline__ Result draw_listed(ListShared<BT>& s, uint32_t m, con
 template <int BT>
 __device__ __forceinline__ Result draw_list(ListShared<BT>& s, uint32_t n, const Settings& o, double u) {
   if (n > 64) return draw_listed<BT>(s, n, o, u);
-  return threadIdx.x < 64 ? draw_wave(threadIdx.x < n ? s.list[threadIdx.x] : LIST_END, n, o, u) : nothing_to_draw();
+  return threadIdx.x < 64 ? draw_wave(s.list, n, o, u) : nothing_to_draw();
 }
 // Greedy: the first of the order among n listed entries.
 template <int BT>
@@ -476,26 +502,29 @@ struct Reader {
   __device__ __forceinline__ uint32_t first(F f, G odd) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) most[i] = 0;
+    uint4 w[2][AHEAD];  // those that are worked on, and those that are under way
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) w[0][i] = load(i * STEP + threadIdx.x * N);
 #pragma unroll 1
     for (uint32_t turn = 0; turn < whole; turn += TURN) {
 #pragma unroll
-      for (int h = 0; h < PIECES; h += AHEAD) {
-        if (turn + h * STEP >= whole) break;
-        uint4 w[AHEAD];
+      for (int h = 0; h < PIECES / AHEAD; ++h) {
+        const uint32_t base = turn + h * AHEAD * STEP;
+        if (base >= whole) break;
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) w[i] = load(turn + (h + i) * STEP + threadIdx.x * N);
+        for (int i = 0; i < AHEAD; ++i) w[1 - h % 2][i] = load(base + (AHEAD + i) * STEP + threadIdx.x * N);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           __builtin_amdgcn_sched_barrier(0);  // pieces are worked on as they arrive: all at once they would not fit the registers
-          const uint32_t c = turn + (h + i) * STEP + threadIdx.x * N;
+          const uint32_t c = base + i * STEP + threadIdx.x * N;
           if (c < whole) {
-            const uint4 p = raw_places<T>(w[i]);
+            const uint4 p = raw_places<T>(w[h % 2][i]);
             uint32_t m = piece_max<T>(p);
             if (m <= P::LARGEST && piece_min<T>(p) > P::LOWEST)
               f(p);
             else
-              m = odd(w[i], c);
-            most[h + i] = max(most[h + i], m);
+              m = odd(w[h % 2][i], c);
+            most[h * AHEAD + i] = max(most[h * AHEAD + i], m);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -507,8 +536,9 @@ struct Reader {
     for (int i = 0; i < PIECES; ++i) m = max(m, most[i]);
     return max(m == P::SIGN - 1 ? P::SIGN : m, last);  // -0
   }
-  // f(piece's bits, column) for every piece that `wanted` (of its raw places) says yes to, of those whose largest place may reach `least`.  They
-  // are read again, one a thread when they are few.  Called by all threads; a barrier is left to the caller.
+  // f(place, column) for every entry of the pieces that `wanted` (of a piece's raw places) says yes to, of those whose largest place may
+  // reach `least`, and perhaps of others.  Pieces that the maxima name are few, or all are read again and those that are wanted are
+  // few; either way an entry of them goes to a thread.  Called by all threads; a barrier is left to the caller.
   template <typename W, typename F>
   __device__ __forceinline__ void again(Shared& s, uint32_t least, W wanted, F f) const {
     const uint32_t raw = least == P::SIGN ? P::SIGN - 1 : least;
@@ -522,32 +552,42 @@ struct Reader {
         if (at < HITS) s.hit[at] = (i * THREADS + threadIdx.x) * N;
       }
     __syncthreads();
-    const uint32_t hits = s.hits;
-    if (hits <= HITS) {
-      if (threadIdx.x < hits)
-        for (uint32_t c = s.hit[threadIdx.x]; c < whole; c += TURN) {
-          const uint4 w = load_words(x + c);
-          if (wanted(raw_places<T>(w))) f(w, c);
-        }
-    } else {
+    uint32_t hits = s.hits, step = TURN;
+    if (hits > HITS) {
+      __syncthreads();
+      if (threadIdx.x == 0) s.hits = 0;
+      __syncthreads();
 #pragma unroll 1
-      for (uint32_t c = threadIdx.x * N; c < whole; c += AHEAD * STEP) {
-        uint4 w[AHEAD];
+      for (uint32_t c = threadIdx.x * N; c < whole; c += 8 * STEP) {
+        uint4 w[8];
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) w[i] = load(c + i * STEP);
+        for (uint32_t i = 0; i < 8; ++i) w[i] = load(c + i * STEP);
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i)
-          if (c + i * STEP < whole && wanted(raw_places<T>(w[i]))) f(w[i], c + i * STEP);
+        for (uint32_t i = 0; i < 8; ++i) {
+          const uint32_t at_column = c + i * STEP;
+          if (at_column < whole && wanted(raw_places<T>(w[i]))) {
+            const uint32_t at = atomicAdd(&s.hits, 1u);
+            if (at < HITS)
+              s.hit[at] = at_column;
+            else
+              each<T>(w[i], at_column, f);  // not few
+          }
+        }
       }
+      __syncthreads();
+      hits = min(s.hits, HITS);
+      step = whole;
     }
+    for (uint32_t i = threadIdx.x; i < hits * N; i += THREADS)
+      for (uint32_t c = s.hit[i / N] + i % N; c < whole; c += step) f(place_of(x[c]), c);
   }
   // f(place, column) for the entries from `least` on
   template <typename F>
   __device__ __forceinline__ void from(Shared& s, uint32_t least, F f) const {
     const uint32_t raw = least == P::SIGN ? P::SIGN - 1 : least;
-    again(s, least, [&](uint4 p) { return piece_max<T>(p) >= raw; },
-          [&](uint4 w, uint32_t c) { each<T>(w, c, [&](uint32_t q, uint32_t col) { if (q >= least) f(q, col); }); });
-    if (last >= least) f(last, whole + threadIdx.x);
+    auto some = [&](uint32_t q, uint32_t c) { if (q >= least) f(q, c); };
+    again(s, least, [&](uint4 p) { return piece_max<T>(p) >= raw; }, some);
+    if (last) some(last, whole + threadIdx.x);
   }
   // f(column) for the entries of a place
   template <typename F>
@@ -555,23 +595,24 @@ struct Reader {
     // what is 0 in a word that holds the place's raw bits; two kinds of bits are the place of 0 and that of the largest number
     const uint32_t other = place == P::SIGN ? P::SIGN - 1 : place == P::LARGEST ? P::LARGEST + 1 : place;
     const uint32_t a = sizeof(T) == 4 ? place : place | place << 16, b = sizeof(T) == 4 ? other : other | other << 16;
+    auto some = [&](uint32_t q, uint32_t c) { if (q == place) f(c); };
     again(s, place, [&](uint4 p) {
       uint32_t m = piece_min<T>(uint4{p.x ^ a, p.y ^ a, p.z ^ a, p.w ^ a});
       if (a != b) m = min(m, piece_min<T>(uint4{p.x ^ b, p.y ^ b, p.z ^ b, p.w ^ b}));
       return m == 0;
-    }, [&](uint4 w, uint32_t c) { each<T>(w, c, [&](uint32_t q, uint32_t col) { if (q == place) f(col); }); });
-    if (last == place) f(whole + threadIdx.x);
+    }, some);
+    if (last) some(last, whole + threadIdx.x);
   }
   // f(value, column) for every entry that is there: later readings of the whole row
   template <typename F>
   __device__ __forceinline__ void all(F f) const {
 #pragma unroll 1
-    for (uint32_t c = threadIdx.x * N; c < whole; c += 4 * STEP) {
-      uint4 w[4];
+    for (uint32_t c = threadIdx.x * N; c < whole; c += 8 * STEP) {
+      uint4 w[8];
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) w[i] = load(c + i * STEP);
+      for (uint32_t i = 0; i < 8; ++i) w[i] = load(c + i * STEP);
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
+      for (uint32_t i = 0; i < 8; ++i) {
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t at = c + i * STEP;
         if (at < whole) {
@@ -634,7 +675,7 @@ __device__ __forceinline__ uint32_t count_of(const Counters& c, uint32_t q) {
 struct Values {
   uint32_t q;         // place of the largest; the others follow downwards
   uint32_t count[4];
-  uint64_t mass[4];   // of all entries of the value
+  uint64_t each[4], mass[4];  // units of an entry of the value, and of all of them
   __device__ __forceinline__ uint32_t counts() const { return count[0] + count[1] + count[2] + count[3]; }
   __device__ __forceinline__ uint64_t masses() const { return mass[0] + mass[1] + mass[2] + mass[3]; }
 };
@@ -651,14 +692,17 @@ __device__ __forceinline__ bool values_of(const Counters& c, uint32_t chunk, Val
 template <typename T>
 __device__ __forceinline__ void weigh(const Row& row, Values* v) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v->mass[j] = v->count[j] ? v->count[j] * row.units(Places<T>::value(v->q - j)) : 0;
+  for (int j = 0; j < 4; ++j) v->each[j] = row.units(v->count[j] ? Places<T>::value(v->q - j) : row.zmax);  // without branches: beside one another
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v->mass[j] = v->count[j] * v->each[j];
 }
 // The value that holds a unit (RANK: of the count; else of mass), from the sums of chunks before each thread's own (thread t < CHUNKS has
 // the t-th chunk from the top).
 struct ValuePlace {
   uint32_t q, tie;
   float z;
-  uint64_t count_before, mass_before;  // of the value
+  uint64_t count_before, mass_before, each;  // before the value; of an entry of it
+  __device__ __forceinline__ uint64_t mass_with() const { return mass_before + (uint64_t)(tie + 1) * each; }
 };
 template <bool RANK, typename T>
 __device__ __forceinline__ ValuePlace locate_value(Shared& s, const Row& row, uint64_t unit, uint64_t count_before, uint64_t mass_before) {
@@ -678,7 +722,7 @@ __device__ __forceinline__ ValuePlace locate_value(Shared& s, const Row& row, ui
   values_of(s.counters, s.chunk, &v);
   weigh<T>(row, &v);
   uint64_t counts = s.count_before + group_scan_u32<64>(v.counts()) - v.counts(), masses = s.mass_before + group_scan_u64<64>(v.masses()) - v.masses();
-  ValuePlace p{0, 0, 0.0f, 0, 0};
+  ValuePlace p{0, 0, 0.0f, 0, 0, 0};
   bool here = false;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -688,6 +732,7 @@ __device__ __forceinline__ ValuePlace locate_value(Shared& s, const Row& row, ui
       p.q = v.q - j;
       p.count_before = counts;
       p.mass_before = masses;
+      p.each = v.each[j];
     }
     counts += v.count[j];
     masses += v.mass[j];
@@ -696,8 +741,9 @@ __device__ __forceinline__ ValuePlace locate_value(Shared& s, const Row& row, ui
   p.q = (uint32_t)__shfl((int)p.q, lane, 64);
   p.count_before = shfl_u64(p.count_before, lane);
   p.mass_before = shfl_u64(p.mass_before, lane);
+  p.each = shfl_u64(p.each, lane);
   p.z = Places<T>::value(p.q);
-  p.tie = RANK ? (uint32_t)(unit - p.count_before) : (uint32_t)((unit - p.mass_before) / row.units(p.z));
+  p.tie = RANK ? (uint32_t)(unit - p.count_before) : Row::quotient(unit - p.mass_before, p.each);
   return p;
 }
 // The largest place up to `most` whose value fails `passes`, which holds from some place on; what is not there fails.
@@ -761,12 +807,12 @@ __device__ __forceinline__ bool draw_by_value(const Reader<T>& in, Shared& s, co
     count = o.top_k;
     if (o.top_k < above) {
       const ValuePlace p = locate_value<true, T>(s, row, o.top_k - 1, count_before, mass_before);
-      mass = p.mass_before + (uint64_t)(p.tie + 1) * row.units(p.z);
+      mass = p.mass_with();
     }
   }
   if (o.top_p < 1.0f) {
     const ValuePlace p = locate_value<false, T>(s, row, Row::needed(o.top_p, mass) - 1, count_before, mass_before);
-    mass = p.mass_before + (uint64_t)(p.tie + 1) * row.units(p.z);
+    mass = p.mass_with();
     count = (uint32_t)p.count_before + p.tie + 1;
   }
   if (o.min_p > 0.0f) {
@@ -810,6 +856,11 @@ struct Bins {
     narrow = scale > 1e-30 && scale < 1e30 ? (float)scale : 0.0f;
   }
   __device__ __forceinline__ bool has(float z) const { return z <= top && z >= low; }
+  // no value of bins 0 .. b is smaller
+  __device__ __forceinline__ float edge(uint32_t b) const {
+    const double z = scale > 0.0 ? hi - ((double)b + 1.0) / scale : (double)low;
+    return fmaxf((float)(z - 1e-5 * fabs(z) - 1e-5 * ((double)top - z)), low);
+  }
   __device__ __forceinline__ uint32_t of(float z) const {
     return min(narrow != 0.0f ? (uint32_t)((top - z) * narrow) : (uint32_t)((hi - (double)z) * scale), BINS - 1);
   }
@@ -819,7 +870,7 @@ struct Bins {
 struct Place {
   float z;
   uint32_t tie, ties, column;
-  uint64_t before;
+  uint64_t before, larger;  // `larger`: entries before the value
 };
 // What a thread knows of the bins it owns, 2 t and 2 t + 1.
 struct Filled {
@@ -870,14 +921,22 @@ __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Ro
     __syncthreads();
     const uint32_t b = s.found;
     before = s.mass_before;
-    // the bin's entries: how many, between which values, and the list of them if it holds them
+    // the bin's entries: how many, between which values, and the list of them if it holds them; and how many entries are larger
     uint32_t kmin = 0xFFFFFFFFu, kmax = 0;
-    in.all([&](float z, uint32_t c) {
-      if (bins.has(z) && bins.of(z) == b) {
-        const uint32_t key = score_key(z), at = atomicAdd(&s.l.n, 1u);
-        kmin = min(kmin, key);
-        kmax = max(kmax, key);
-        if (at < CAP) s.l.list[at] = listed(z, c);
+    uint64_t larger = 0;
+    in.from(s, place_of((T)bins.edge(b)), [&](uint32_t q, uint32_t c) {
+      const float z = Places<T>::value(q);
+      if (z > bins.top) {
+        ++larger;
+      } else if (z >= bins.low) {
+        const uint32_t mine = bins.of(z);
+        larger += mine < b;
+        if (mine == b) {
+          const uint32_t key = score_key(z), at = atomicAdd(&s.l.n, 1u);
+          kmin = min(kmin, key);
+          kmax = max(kmax, key);
+          if (at < CAP) s.l.list[at] = listed(z, c);
+        }
       }
     });
     kmin = wave_min_u32(kmin);
@@ -886,11 +945,11 @@ __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Ro
       atomicMin(&s.lo, kmin);
       atomicMax(&s.hi, kmax);
     }
-    __syncthreads();
+    block_scan<THREADS>(larger, s.wave, &p.larger);  // its barriers publish the list
     const uint32_t n = s.l.n;
     const float lo = key_score(s.lo), hi = key_score(s.hi);
     if (lo == hi) {  // one value: the place among its equals
-      p = Place{hi, (uint32_t)((unit - before) / value(hi)), n, SKY_INVALID, before};
+      p = Place{hi, Row::quotient(unit - before, value(hi)), n, SKY_INVALID, before, p.larger};
       if (n == 1) p.column = (uint32_t)s.l.list[0];
       return p;
     }
@@ -917,6 +976,7 @@ __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Ro
       p.ties = (uint32_t)ties;
       p.tie = s.found - (uint32_t)s.count_before;
       p.before = s.mass_before;
+      p.larger += s.count_before;
       return p;
     }
     bins = Bins(hi, lo);
@@ -953,10 +1013,7 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, c
     const Place p = locate<false>(in, s, row, bins, f, low, excess, Row::needed(o.top_p, mass) - 1);
     mass = p.before + (uint64_t)(p.tie + 1) * row.units(p.z);
     end = p.z;
-    uint64_t larger = 0, all;
-    in.all([&](float z, uint32_t) { larger += z > end; });
-    block_scan<THREADS>(larger, s.wave, &all);
-    count = (uint32_t)all + p.tie + 1;
+    count = (uint32_t)p.larger + p.tie + 1;
   }
   if (o.min_p > 0.0f && (row.weight(end) < (double)o.min_p || (cut_off && !(o.top_p < 1.0f)))) {
     const uint32_t least = min(last_failing<T>(most, [&](float z) { return row.weight(z) >= (double)o.min_p; }) + 1, most);
