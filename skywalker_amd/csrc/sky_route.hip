@@ -71,6 +71,8 @@ __device__ __forceinline__ bool open_expert(float x) { return x > -__builtin_inf
 // log(1 / (1 + exp(-x)))
 __device__ __forceinline__ double log_sigmoid(double x) { return fmin(x, 0.0) - log1p(exp(-fabs(x))); }
 
+__device__ __forceinline__ bool chosen_by_logit(const sky_route_rules& r) { return !r.bias && !(r.groups > 1 && r.groups_kept < r.groups && r.group_top2); }
+
 // The choice of one row in fp64, into lanes first + j.  Keys: 0 is a closed expert, a taken one or none.
 template <typename T, int PER>
 __device__ __forceinline__ uint32_t choose_exactly(const T* x, const RouteArgs& a, double* staged, uint32_t first, uint32_t id) {
@@ -83,7 +85,8 @@ __device__ __forceinline__ uint32_t choose_exactly(const T* x, const RouteArgs& 
   }
   zmax = wave_max_f32(zmax);
   double sum = 0.0;
-  if (!a.r.sigmoid) {
+  const bool by_logit = chosen_by_logit(a.r);
+  if (!a.r.sigmoid && !by_logit) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) sum += open_expert(z[i]) ? exp((double)z[i] - (double)zmax) : 0.0;
     sum = group_sum_f64<64>(sum);
@@ -94,7 +97,7 @@ __device__ __forceinline__ uint32_t choose_exactly(const T* x, const RouteArgs& 
     const uint32_t e = lane * PER + i;
     key[i] = 0;
     if (open_expert(z[i])) {
-      const double score = a.r.sigmoid ? 1.0 / (1.0 + exp(-(double)z[i])) : exp((double)z[i] - (double)zmax) / sum;
+      const double score = by_logit ? (double)z[i] : a.r.sigmoid ? 1.0 / (1.0 + exp(-(double)z[i])) : exp((double)z[i] - (double)zmax) / sum;
       key[i] = double_key(score + (a.r.bias ? (double)a.r.bias[e] : 0.0));
     }
   }
@@ -152,6 +155,292 @@ __device__ __forceinline__ uint32_t choose_exactly(const T* x, const RouteArgs& 
   return id;
 }
 
+// The weights of the wavefront's rows, a chosen expert a lane: the j-th of `row`, whose lanes lie together, `slots` of them.
+template <typename T>
+__device__ __forceinline__ void store_weights(const RouteArgs& a, uint32_t row, bool real, uint32_t j, uint32_t slots, uint32_t id, float zmax, double sum) {
+  const uint32_t k = a.r.k;
+  const bool mine = real && j < k, in = mine && id != SKY_INVALID;
+  const float chosen = in ? plain_score((float)((const T*)a.logits + row * a.stride)[id]) : 0.0f;
+  double w = 0.0;
+  if (a.r.renormalise) {
+    // the first of the order has not got the largest score when a bias or groups decide
+    const double l = !in ? 0.0 : a.r.sigmoid ? log_sigmoid(chosen) : (double)chosen;
+    double most = in ? l : -__builtin_inf();
+    for (uint32_t m = 1; m < slots; m *= 2) most = fmax(most, __shfl_xor(most, (int)m, 64));
+    w = in ? exp(l - most) : 0.0;
+    double all = w;
+    for (uint32_t m = 1; m < slots; m *= 2) all += __shfl_xor(all, (int)m, 64);
+    w = all > 0.0 ? w / all : 0.0;
+  } else if (in) {
+    w = a.r.sigmoid ? 1.0 / (1.0 + exp(-(double)chosen)) : exp((double)chosen - (double)zmax) / sum;
+  }
+  if (mine) {
+    a.ids[(uint64_t)row * k + j] = id;
+    a.weights[(uint64_t)row * k + j] = in ? (float)((double)a.r.scale * w) : 0.0f;
+  }
+}
+
+// ---------------------------------------------------------------- four rows at a time
+// Up to 256 experts, 16 chosen and 16 groups: 16 lanes have a row, lane l of them the experts PER l, PER l + 1, ...  The k best are not
+// taken out one after another: the k-th largest of the lanes' largest is no larger than the k-th largest of all, some 11 of 256
+// experts reach the 8th, and each of those counts how many come before it.  Everything a row asks of its lanes are rotations within 16
+// lanes, which cost an instruction.
+constexpr int QUAD_EXPERTS = 256, QUAD_K = 16, QUAD_GROUPS = 16;
+constexpr uint32_t QUAD_LISTED = 128;  // candidates of a row; a row with more (many equal ones) is chosen from in fp64, one by one
+
+template <int N>
+__device__ __forceinline__ uint32_t turn16(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xF, 0xF, true);  // from lane (l - N) mod 16
+}
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+  v = max(v, turn16<8>(v));
+  v = max(v, turn16<4>(v));
+  v = max(v, turn16<2>(v));
+  return max(v, turn16<1>(v));
+}
+__device__ __forceinline__ uint32_t min16(uint32_t v) { return ~max16(~v); }
+__device__ __forceinline__ float sum16(float v) {
+  v += __uint_as_float(turn16<8>(__float_as_uint(v)));
+  v += __uint_as_float(turn16<4>(__float_as_uint(v)));
+  v += __uint_as_float(turn16<2>(__float_as_uint(v)));
+  return v + __uint_as_float(turn16<1>(__float_as_uint(v)));
+}
+__device__ __forceinline__ uint32_t prefix16(uint32_t v) { return group_scan_u32<16>(v); }
+// How many of the 16 lanes hold more; with `or_equal_before`, equal ones of smaller lanes too.
+template <int N = 1>
+__device__ __forceinline__ uint32_t larger16(uint32_t v, uint32_t sub, bool or_equal_before) {
+  const uint32_t o = turn16<N>(v);
+  const uint32_t mine = o > v || (or_equal_before && o == v && sub >= N);  // lane (l - N) mod 16 is smaller than l where l >= N
+  if constexpr (N < 15)
+    return mine + larger16<N + 1>(v, sub, or_equal_before);
+  else
+    return mine;
+}
+// e^x of x <= 0, to some 1e-14
+__device__ __forceinline__ double exp_negative(double x) {
+  const double t = fmax(x * 1.44269504088896340736, -1000.0), n = rint(t), f = (t - n) * 0.69314718055994530942;
+  double p = 1.0 / 39916800.0;
+  p = fma(p, f, 1.0 / 3628800.0);
+  p = fma(p, f, 1.0 / 362880.0);
+  p = fma(p, f, 1.0 / 40320.0);
+  p = fma(p, f, 1.0 / 5040.0);
+  p = fma(p, f, 1.0 / 720.0);
+  p = fma(p, f, 1.0 / 120.0);
+  p = fma(p, f, 1.0 / 24.0);
+  p = fma(p, f, 1.0 / 6.0);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  return __longlong_as_double(__double_as_longlong(p) + ((long long)(int)n << 52));
+}
+
+template <typename T, int PER>
+__global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteArgs a, uint32_t turns, uint32_t slots) {
+  constexpr int WIDE = PER > 4 ? PER / 4 : 1;  // experts a lane where a wavefront has a row
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & 15, quarter = lane >> 4;
+  const uint32_t row0 = (blockIdx.x * ROUTE_WAVES + wave) * (4 * turns), E = a.experts, k = a.r.k;
+  struct Wave {
+    union {
+      uint32_t key[4][16 * PER];  // of the four rows, where groups are not whole lanes
+      struct {
+        float listed[4][QUAD_LISTED + 4];  // choices (logits where it goes by them), filled up to four with what is none
+        uint32_t expert[4][QUAD_LISTED];
+      };
+      double exact[64 * WIDE];
+    };
+    uint32_t id[64];  // chosen: row n of the wavefront has slots n * slots ...
+    double sum[64];
+    float zmax[64];
+  };
+  __shared__ Wave shared[ROUTE_WAVES];
+  if (row0 >= a.rows) return;
+  Wave& s = shared[wave];
+  const uint32_t rows = min(4 * turns, a.rows - row0);
+  const bool grouped = a.r.groups > 1 && a.r.groups_kept < a.r.groups;
+  const bool by_logit = chosen_by_logit(a.r);
+  const bool full_sum = !a.r.sigmoid && !a.r.renormalise;
+  const uint32_t size = E / a.r.groups, lanes = size / PER;  // of a group
+  const bool whole_lanes = size % PER == 0 && (lanes & (lanes - 1)) == 0;
+  float bias[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) bias[i] = a.r.bias && sub * PER + i < E ? a.r.bias[sub * PER + i] : 0.0f;
+  s.id[lane] = SKY_INVALID;
+  for (uint32_t t = 0; t < turns; ++t) {
+    const uint32_t n = 4 * t + quarter;  // of the wavefront's rows
+    if (4 * t >= rows) break;
+    const T* const x = (const T*)a.logits + (uint64_t)(row0 + min(n, rows - 1)) * a.stride;
+    float z[PER];
+    if (PER * 16 == E) {
+      T v[PER];
+      __builtin_memcpy(v, x + sub * PER, sizeof(v));
+#pragma unroll
+      for (int i = 0; i < PER; ++i) z[i] = plain_score((float)v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) z[i] = sub * PER + i < E ? plain_score((float)x[sub * PER + i]) : -__builtin_inff();
+    }
+    float zmax = z[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) zmax = fmaxf(zmax, z[i]);
+    zmax = key_score(max16(score_key(zmax)));
+    if (full_sum) {
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const double w = exp_negative((double)z[i] - (double)zmax);
+        sum += open_expert(z[i]) ? w : 0.0;
+      }
+      sum = group_sum_f64<16>(sum);
+      if (sub == 0) {
+        s.sum[n] = sum;
+        s.zmax[n] = zmax;
+      }
+    }
+    uint32_t key[PER];
+    float near = 0.0f;  // choices that are nearer than this may be the other way round
+    if (by_logit) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) key[i] = open_expert(z[i]) ? score_key(z[i]) : 0;
+    } else {
+      // Scores: the exponent's product is off by 2^-24 of itself, which its size times the score bounds by 0.53, exponential, sum and
+      // quotient by some 2^-22: less than 2^-20 of the largest score in all.  The sum with the bias: 2^-24.
+      float c[PER], most = 1.0f;
+      if (a.r.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) c[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fminf(-z[i] * 1.44269504f, 126.0f)));
+      } else {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          c[i] = open_expert(z[i]) ? __builtin_amdgcn_exp2f((z[i] - zmax) * 1.44269504f) : 0.0f;
+          sum += c[i];
+        }
+        most = __builtin_amdgcn_rcpf(sum16(sum));
+#pragma unroll
+        for (int i = 0; i < PER; ++i) c[i] *= most;
+      }
+      float size_of_choice = 0.0f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        c[i] += bias[i];
+        size_of_choice = fmaxf(size_of_choice, fabsf(c[i]));
+        key[i] = open_expert(z[i]) ? score_key(c[i]) : 0;
+      }
+      near = 0x1p-18f * most + 0x1p-22f * key_score(max16(score_key(size_of_choice)));
+    }
+    bool doubt = false;  // of this lane
+    if (grouped) {
+      uint32_t best = 0, second = 0, owner;  // owner: the lane that speaks for this lane's experts
+      if (whole_lanes) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          second = max(second, min(best, key[i]));
+          best = max(best, key[i]);
+        }
+        for (uint32_t m = 1; m < lanes; m *= 2) {
+          const uint32_t b = (uint32_t)__shfl_xor((int)best, (int)m, 64), c = (uint32_t)__shfl_xor((int)second, (int)m, 64);
+          second = max(min(best, b), max(second, c));
+          best = max(best, b);
+        }
+        owner = sub & ~(lanes - 1);
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) s.key[quarter][sub * PER + i] = key[i];
+        __builtin_amdgcn_wave_barrier();
+        if (sub < a.r.groups)
+          for (uint32_t i = 0; i < size; ++i) {
+            const uint32_t v = s.key[quarter][sub * size + i];
+            second = max(second, min(best, v));
+            best = max(best, v);
+          }
+        __builtin_amdgcn_wave_barrier();
+        owner = sub;
+      }
+      uint32_t mine = best;
+      if (best && second && a.r.group_top2) mine = score_key(key_score(best) + key_score(second));
+      if (owner != sub) mine = 0;
+      const bool stays = mine && larger16(mine, sub, true) < a.r.groups_kept;
+      const uint32_t last = min16(stays ? mine : 0xFFFFFFFFu), next = max16(stays ? 0 : mine);
+      if (!by_logit && next) doubt = !(key_score(last) - key_score(next) > 4.0f * near);
+      const uint32_t stay = (uint32_t)(__ballot(stays) >> (lane & 48)) & 0xFFFFu;
+      if (whole_lanes) {
+        const bool mine_stays = stay >> owner & 1;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) key[i] = mine_stays ? key[i] : 0;
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const uint32_t e = sub * PER + i;
+          if (e >= E || !(stay >> (e / size) & 1)) key[i] = 0;
+        }
+      }
+    }
+    // candidates: what reaches the k-th largest of the lanes' largest, or may
+    uint32_t top = key[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) top = max(top, key[i]);
+    uint32_t least = min16(larger16(top, sub, false) < k ? top : 0xFFFFFFFFu);
+    if (!by_logit && least) least = score_key(key_score(least) - 2.0f * near);
+    least = max(least, 1u);
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += key[i] >= least;
+    const uint32_t sum = prefix16(mine), count = (uint32_t)__shfl((int)sum, (int)(lane | 15), 64);
+    if (count > QUAD_LISTED) doubt = true;
+    uint32_t at = sum - mine;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] >= least) {
+        if (at < QUAD_LISTED) {
+          s.listed[quarter][at] = key_score(key[i]);
+          s.expert[quarter][at] = sub * PER + i;
+        }
+        ++at;
+      }
+    const uint32_t listed = min(count, QUAD_LISTED);
+    if (sub < 4) s.listed[quarter][listed + sub] = -__builtin_inff();
+    __builtin_amdgcn_wave_barrier();
+    for (uint32_t c = sub; c < listed; c += 16) {
+      const float v = s.listed[quarter][c];
+      uint32_t rank = 0, close = 0;
+      for (uint32_t j = 0; j < listed; j += 4) {
+        const float4 o = *(const float4*)&s.listed[quarter][j];
+        const float four[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          rank += four[i] > v || (four[i] == v && j + i < c);
+          close += fabsf(four[i] - v) <= 2.0f * near;  // itself among them
+        }
+      }
+      const uint32_t e = s.expert[quarter][c];
+      if (rank < k) {
+        if (!by_logit && close > 1)
+          for (uint32_t j = 0; j < listed; ++j)
+            if (fabsf(s.listed[quarter][j] - v) <= 2.0f * near) {
+              // alike, the same logit and bias, they stand as they are
+              const uint32_t f = s.expert[quarter][j];
+              doubt |= !((float)x[e] == (float)x[f] && (!a.r.bias || a.r.bias[e] == a.r.bias[f]));
+            }
+        if (n < rows) s.id[n * slots + rank] = e;
+      }
+    }
+    // rows in doubt, one after another by the whole wavefront
+    uint64_t rest = __ballot(doubt);
+    while (rest) {
+      const uint32_t q = (uint32_t)__builtin_ctzll(rest) >> 4, m = 4 * t + q;
+      rest &= ~(0xFFFFull << (16 * q));
+      if (m >= rows) continue;
+      __builtin_amdgcn_wave_barrier();
+      const uint32_t id = choose_exactly<T, WIDE>((const T*)a.logits + (uint64_t)(row0 + m) * a.stride, a, s.exact, 0, SKY_INVALID);
+      if (lane < slots) s.id[m * slots + lane] = id;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  const uint32_t n = lane / slots;
+  store_weights<T>(a, row0 + n, n < rows, lane % slots, slots, s.id[lane], full_sum ? s.zmax[n] : 0.0f, full_sum ? s.sum[n] : 1.0);
+}
+
+// ---------------------------------------------------------------- a row at a time
 // A wavefront takes rows_per_wave rows, which fill it with chosen experts: `slots` lanes (a power of two, at least k) for a row's.
 template <typename T, int PER>
 __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, uint32_t rows_per_wave, uint32_t slots) {
@@ -162,7 +451,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
   double* const staged = staged_all[wave];
   const uint32_t rows = min(rows_per_wave, a.rows - row0);
   const bool grouped = a.r.groups > 1 && a.r.groups_kept < a.r.groups;
-  const bool by_logit = !a.r.bias && !(grouped && a.r.group_top2);
+  const bool by_logit = chosen_by_logit(a.r);
   const bool full_sum = !a.r.sigmoid && !a.r.renormalise;  // the sum over all experts goes into the weights
   const uint32_t size = E / a.r.groups, lanes = size / PER;  // of a group
   // groups whose experts are whole lanes, a power of two of them, are reduced across lanes; others through LDS
@@ -312,27 +601,8 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
       id = choose_exactly<T, PER>(x, a, staged, first, id);
     }
   }
-  // the weights of all of the wavefront's rows: lane n * slots + j has the j-th of row n
-  const uint32_t n = lane / slots, j = lane % slots;
-  const bool mine = n < rows && j < k, in = mine && id != SKY_INVALID;
-  const float chosen = in ? plain_score((float)((const T*)a.logits + (row0 + n) * a.stride)[id]) : 0.0f;
-  double w = 0.0;
-  if (a.r.renormalise) {
-    // the first of the order has not got the largest score when a bias or groups decide
-    const double l = !in ? 0.0 : a.r.sigmoid ? log_sigmoid(chosen) : (double)chosen;
-    double most = in ? l : -__builtin_inf();
-    for (uint32_t m = 1; m < slots; m *= 2) most = fmax(most, __shfl_xor(most, (int)m, 64));
-    w = in ? exp(l - most) : 0.0;
-    double all = w;
-    for (uint32_t m = 1; m < slots; m *= 2) all += __shfl_xor(all, (int)m, 64);
-    w = all > 0.0 ? w / all : 0.0;
-  } else if (in) {
-    w = a.r.sigmoid ? 1.0 / (1.0 + exp(-(double)chosen)) : exp((double)chosen - (double)my_max) / my_sum;
-  }
-  if (mine) {
-    a.ids[(uint64_t)(row0 + n) * k + j] = id;
-    a.weights[(uint64_t)(row0 + n) * k + j] = in ? (float)((double)a.r.scale * w) : 0.0f;
-  }
+  const uint32_t n = lane / slots;
+  store_weights<T>(a, row0 + n, n < rows, lane % slots, slots, id, my_max, my_sum);
 }
 
 constexpr int COUNT_THREADS = 1024;
@@ -444,10 +714,16 @@ int check_route(const char* who, uint32_t rows, uint32_t experts, const sky_rout
    : experts <= 256 ? launch(kernel<T, 4>)                                                \
    : experts <= 512 ? launch(kernel<T, 8>)                                                \
                     : launch(kernel<T, 16>))
-#define SKY_ROUTE_LAUNCH(kernel)                       \
-  (dtype == SKY_F32 ? SKY_ROUTE_PER(kernel, float)     \
-   : dtype == SKY_F16 ? SKY_ROUTE_PER(kernel, _Float16) \
-                      : SKY_ROUTE_PER(kernel, __bf16))
+#define SKY_ROUTE_QUAD(kernel, T)                                                         \
+  (experts <= 16 ? launch(kernel<T, 1>)                                                   \
+   : experts <= 32 ? launch(kernel<T, 2>)                                                 \
+   : experts <= 64 ? launch(kernel<T, 4>)                                                 \
+   : experts <= 128 ? launch(kernel<T, 8>)                                                \
+                    : launch(kernel<T, 16>))
+#define SKY_ROUTE_LAUNCH(PER, kernel)       \
+  (dtype == SKY_F32 ? PER(kernel, float)    \
+   : dtype == SKY_F16 ? PER(kernel, _Float16) \
+                      : PER(kernel, __bf16))
 
 }  // namespace
 }  // namespace sky
@@ -480,13 +756,24 @@ extern "C" int sky_route_topk(const void* logits, int dtype, uint32_t rows, uint
   a.weights = weights;
   uint32_t slots = 1;
   while (slots < rules->k) slots *= 2;
-  // as many rows a wavefront as fill it with chosen experts, as long as there is a wavefront for every SIMD
-  const uint32_t per_wave = std::min(64 / slots, std::max(rows / 2048u, 1u));
-  const uint64_t waves = ((uint64_t)rows + per_wave - 1) / per_wave;
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)((waves + ROUTE_WAVES - 1) / ROUTE_WAVES)), dim3(64 * ROUTE_WAVES), 0, st, a, per_wave, slots);
-  };
-  SKY_ROUTE_LAUNCH(route_kernel);
+  if (experts <= QUAD_EXPERTS && rules->k <= QUAD_K && rules->groups <= QUAD_GROUPS) {
+    // four rows at a time, as many times as fill the wavefront with chosen experts, as long as there are wavefronts for every SIMD
+    slots = std::max(slots, 4u);
+    const uint32_t turns = std::min(16 / slots, std::max(rows / 8192u, 1u));
+    const uint32_t per_block = 4 * turns * ROUTE_WAVES;
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((rows + per_block - 1) / per_block), dim3(64 * ROUTE_WAVES), 0, st, a, turns, slots);
+    };
+    SKY_ROUTE_LAUNCH(SKY_ROUTE_QUAD, route_quad_kernel);
+  } else {
+    // as many rows a wavefront as fill it with chosen experts, as long as there is a wavefront for every SIMD
+    const uint32_t per_wave = std::min(64 / slots, std::max(rows / 2048u, 1u));
+    const uint64_t waves = ((uint64_t)rows + per_wave - 1) / per_wave;
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((uint32_t)((waves + ROUTE_WAVES - 1) / ROUTE_WAVES)), dim3(64 * ROUTE_WAVES), 0, st, a, per_wave, slots);
+    };
+    SKY_ROUTE_LAUNCH(SKY_ROUTE_PER, route_kernel);
+  }
   if (counts) {
     const uint64_t n = (uint64_t)rows * rules->k;
     hipLaunchKernelGGL(clear_counts_kernel, dim3((experts + 255) / 256), dim3(256), 0, st, counts, experts);
@@ -522,6 +809,6 @@ extern "C" int sky_route_topk_backward(const void* logits, int dtype, uint32_t r
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((rows + ROUTE_WAVES - 1) / ROUTE_WAVES), dim3(64 * ROUTE_WAVES), 0, st, a);
   };
-  SKY_ROUTE_LAUNCH(route_backward_kernel);
+  SKY_ROUTE_LAUNCH(SKY_ROUTE_PER, route_backward_kernel);
   return check_launch();
 }

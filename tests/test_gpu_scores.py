@@ -378,6 +378,20 @@ def test_route_with_ties_closed_experts_and_extremes(capi, dtype, sigmoid):
         run_route(capi, x, dtype, 6, sigmoid=sigmoid, renormalise=renorm, bias=np.zeros(70, np.float32))
 
 
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_route_of_equal_groups_and_equal_choices(capi, sigmoid):
+    # experts whose scores and biases differ in different last bits, groups that are worth the same, rows of one value
+    x = np.zeros((40, 256), np.float32)
+    x[1:20] = np.float32(2.0) + np.random.default_rng(3).integers(-2, 3, (19, 256)) * np.float32(2.0 ** -22)
+    x[20:] = np.random.default_rng(4).integers(-3, 4, (20, 256))
+    bias = (np.random.default_rng(5).integers(-2, 3, 256) * 2.0 ** -24).astype(np.float32)
+    for top2 in (False, True):
+        for b in (None, bias, np.zeros(256, np.float32)):
+            for groups, kept, k in ((8, 3, 7), (1, 1, 16), (16, 5, 16), (32, 20, 9), (8, 4, 33)):
+                run_route(capi, x, "f32", k, sigmoid=sigmoid, bias=b, groups=groups, kept=kept, top2=top2)
+                run_route(capi, x[:, :96], "bf16", min(k, 15), sigmoid=sigmoid, bias=None if b is None else b[:96], groups=groups, kept=max(kept, -(-min(k, 15) // (96 // groups))), top2=top2, renormalise=False)
+
+
 def test_route_of_a_long_batch(capi):
     rng = np.random.default_rng(12)
     run_route(capi, rng.normal(0, 2, (20011, 32)).astype(np.float32), "bf16", 4)
