@@ -28,6 +28,7 @@ struct RouteArgs {
   sky_route_rules r;
   uint32_t* ids;
   float* weights;
+  uint32_t* counts;  // to be cleared by the first workgroup for the kernel that follows; may be null
   const uint32_t* ids_in;
   const float* dweights;
   void* dlogits;
@@ -239,6 +240,8 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
   constexpr int WIDE = PER > 4 ? PER / 4 : 1;  // experts a lane where a wavefront has a row
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & 15, quarter = lane >> 4;
   const uint32_t row0 = (blockIdx.x * ROUTE_WAVES + wave) * (4 * turns), E = a.experts, k = a.r.k;
+  if (blockIdx.x == 0 && a.counts)
+    for (uint32_t e = threadIdx.x; e < E; e += 64 * ROUTE_WAVES) a.counts[e] = 0;
   struct Wave {
     union {
       uint32_t key[4][16 * PER];  // of the four rows, where groups are not whole lanes
@@ -302,8 +305,10 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
 #pragma unroll
       for (int i = 0; i < PER; ++i) key[i] = open_expert(z[i]) ? score_key(z[i]) : 0;
     } else {
-      // Scores: the exponent's product is off by 2^-24 of itself, which its size times the score bounds by 0.53, exponential, sum and
-      // quotient by some 2^-22: less than 2^-20 of the largest score in all.  The sum with the bias: 2^-24.
+      // What fp32 costs.  Sigmoid: constant and product leave the exponent off by 2^-23.4 of itself, the exponential by 2^-23 more, which
+      // moves the score by s (1 - s) of that (0.17 and 0.25 units of 2^-23); sum and reciprocal 1.5 units of s: 2^-22 in all.  Softmax: as much
+      // for each, and their sum, 20 additions deep, off by 12 units of 2^-23 for all alike.  The bias: 2^-24 of the choice.  Two
+      // choices are the right way round if they differ by twice that; `near` is twice as much again.
       float c[PER], most = 1.0f;
       if (a.r.sigmoid) {
 #pragma unroll
@@ -326,7 +331,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
         size_of_choice = fmaxf(size_of_choice, fabsf(c[i]));
         key[i] = open_expert(z[i]) ? score_key(c[i]) : 0;
       }
-      near = 0x1p-18f * most + 0x1p-22f * key_score(max16(score_key(size_of_choice)));
+      near = (a.r.sigmoid ? 0x1p-20f : 0x1p-18f * most) + 0x1p-22f * key_score(max16(score_key(size_of_choice)));
     }
     bool doubt = false;  // of this lane
     if (grouped) {
@@ -361,7 +366,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
       if (owner != sub) mine = 0;
       const bool stays = mine && larger16(mine, sub, true) < a.r.groups_kept;
       const uint32_t last = min16(stays ? mine : 0xFFFFFFFFu), next = max16(stays ? 0 : mine);
-      if (!by_logit && next) doubt = !(key_score(last) - key_score(next) > 4.0f * near);
+      if (!by_logit && next) doubt = !(key_score(last) - key_score(next) > 3.0f * near);
       const uint32_t stay = (uint32_t)(__ballot(stays) >> (lane & 48)) & 0xFFFFu;
       if (whole_lanes) {
         const bool mine_stays = stay >> owner & 1;
@@ -380,7 +385,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
 #pragma unroll
     for (int i = 1; i < PER; ++i) top = max(top, key[i]);
     uint32_t least = min16(larger16(top, sub, false) < k ? top : 0xFFFFFFFFu);
-    if (!by_logit && least) least = score_key(key_score(least) - 2.0f * near);
+    if (!by_logit && least) least = score_key(key_score(least) - near);
     least = max(least, 1u);
     uint32_t mine = 0;
 #pragma unroll
@@ -409,14 +414,14 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
           rank += four[i] > v || (four[i] == v && j + i < c);
-          close += fabsf(four[i] - v) <= 2.0f * near;  // itself among them
+          close += fabsf(four[i] - v) <= near;  // itself among them
         }
       }
       const uint32_t e = s.expert[quarter][c];
       if (rank < k) {
         if (!by_logit && close > 1)
           for (uint32_t j = 0; j < listed; ++j)
-            if (fabsf(s.listed[quarter][j] - v) <= 2.0f * near) {
+            if (fabsf(s.listed[quarter][j] - v) <= near) {
               // alike, the same logit and bias, they stand as they are
               const uint32_t f = s.expert[quarter][j];
               doubt |= !((float)x[e] == (float)x[f] && (!a.r.bias || a.r.bias[e] == a.r.bias[f]));
@@ -446,6 +451,8 @@ template <typename T, int PER>
 __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, uint32_t rows_per_wave, uint32_t slots) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t row0 = (blockIdx.x * ROUTE_WAVES + wave) * rows_per_wave, E = a.experts, k = a.r.k;
+  if (blockIdx.x == 0 && a.counts)
+    for (uint32_t e = threadIdx.x; e < E; e += 64 * ROUTE_WAVES) a.counts[e] = 0;
   __shared__ double staged_all[ROUTE_WAVES][64 * PER];
   if (row0 >= a.rows) return;
   double* const staged = staged_all[wave];
@@ -495,8 +502,10 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
 #pragma unroll
       for (int i = 0; i < PER; ++i) key[i] = open_expert(z[i]) ? score_key(z[i]) : 0;
     } else {
-      // Scores: the exponent's product is off by 2^-24 of itself, which its size times the score bounds by 0.53, exponential, sum and
-      // quotient by some 2^-22: less than 2^-20 of the largest score in all.  The sum with the bias: 2^-24.
+      // What fp32 costs.  Sigmoid: constant and product leave the exponent off by 2^-23.4 of itself, the exponential by 2^-23 more, which
+      // moves the score by s (1 - s) of that (0.17 and 0.25 units of 2^-23); sum and reciprocal 1.5 units of s: 2^-22 in all.  Softmax: as much
+      // for each, and their sum, 20 additions deep, off by 12 units of 2^-23 for all alike.  The bias: 2^-24 of the choice.  Two
+      // choices are the right way round if they differ by twice that; `near` is twice as much again.
       float s[PER], most;
       if (a.r.sigmoid) {
 #pragma unroll
@@ -521,7 +530,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
         key[i] = open_expert(z[i]) ? score_key(c) : 0;
       }
       size_of_choice = key_score(wave_top(score_key(size_of_choice)));
-      near = 0x1p-18f * most + 0x1p-22f * size_of_choice;
+      near = (a.r.sigmoid ? 0x1p-20f : 0x1p-18f * most) + 0x1p-22f * size_of_choice;
     }
     bool exact = true;  // the choice so far
     if (grouped) {
@@ -566,7 +575,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
         if (lane == l) mine = 0;
       }
       const uint32_t next = last ? wave_top(mine) : 0;
-      if (!by_logit && next && !(key_score(last) - key_score(next) > 4.0f * near)) exact = false;
+      if (!by_logit && next && !(key_score(last) - key_score(next) > 3.0f * near)) exact = false;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const uint32_t e = lane * PER + i;
@@ -586,7 +595,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
       if (!best) break;
       const uint32_t winner = (uint32_t)__builtin_ctzll(__ballot(mine == best));  // of equals the first lane, and its first, has the smallest number
       const uint32_t e = (uint32_t)__builtin_amdgcn_readlane((int)(lane * PER + at), (int)winner);
-      if (!by_logit && j && !(key_score(before) - key_score(best) > 2.0f * near))
+      if (!by_logit && j && !(key_score(before) - key_score(best) > near))
         // alike: the same logit and bias
         exact = (float)x[e] == (float)x[before_e] && (!a.r.bias || a.r.bias[e] == a.r.bias[before_e]);
       before = best;
@@ -754,6 +763,7 @@ extern "C" int sky_route_topk(const void* logits, int dtype, uint32_t rows, uint
   a.r = *rules;
   a.ids = ids;
   a.weights = weights;
+  a.counts = counts;
   uint32_t slots = 1;
   while (slots < rules->k) slots *= 2;
   if (experts <= QUAD_EXPERTS && rules->k <= QUAD_K && rules->groups <= QUAD_GROUPS) {
@@ -776,7 +786,6 @@ extern "C" int sky_route_topk(const void* logits, int dtype, uint32_t rows, uint
   }
   if (counts) {
     const uint64_t n = (uint64_t)rows * rules->k;
-    hipLaunchKernelGGL(clear_counts_kernel, dim3((experts + 255) / 256), dim3(256), 0, st, counts, experts);
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((n + 4 * COUNT_THREADS - 1) / (4 * COUNT_THREADS), 64);
     hipLaunchKernelGGL(count_experts_kernel, dim3(blocks), dim3(COUNT_THREADS), 0, st, ids, n, experts, counts);
   }
