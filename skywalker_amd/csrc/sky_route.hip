@@ -69,8 +69,25 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
   return v;
 }
 __device__ __forceinline__ bool open_expert(float x) { return x > -__builtin_inff(); }
-// log(1 / (1 + exp(-x)))
-__device__ __forceinline__ double log_sigmoid(double x) { return fmin(x, 0.0) - log1p(exp(-fabs(x))); }
+// e^x of x <= 0, to some 1e-14: the series of e^f on |f| <= ln(2) / 2 through degree 11
+__device__ __forceinline__ double exp_negative(double x) {
+  const double t = fmax(x * 1.44269504088896340736, -1000.0), n = rint(t), f = (t - n) * 0.69314718055994530942;
+  double p = 1.0 / 39916800.0;
+  p = fma(p, f, 1.0 / 3628800.0);
+  p = fma(p, f, 1.0 / 362880.0);
+  p = fma(p, f, 1.0 / 40320.0);
+  p = fma(p, f, 1.0 / 5040.0);
+  p = fma(p, f, 1.0 / 720.0);
+  p = fma(p, f, 1.0 / 120.0);
+  p = fma(p, f, 1.0 / 24.0);
+  p = fma(p, f, 1.0 / 6.0);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  return __longlong_as_double(__double_as_longlong(p) + ((long long)(int)n << 52));
+}
+// 1 / (1 + exp(-x)) * exp(-m) for m = min(x, 0) or between that and 0: the part of a score that shares hang on
+__device__ __forceinline__ double sigmoid_over(double x, double m) { return exp_negative(fmin(x, 0.0) - m) / (1.0 + exp_negative(-fabs(x))); }
 
 __device__ __forceinline__ bool chosen_by_logit(const sky_route_rules& r) { return !r.bias && !(r.groups > 1 && r.groups_kept < r.groups && r.group_top2); }
 
@@ -164,16 +181,15 @@ __device__ __forceinline__ void store_weights(const RouteArgs& a, uint32_t row, 
   const float chosen = in ? plain_score((float)((const T*)a.logits + row * a.stride)[id]) : 0.0f;
   double w = 0.0;
   if (a.r.renormalise) {
-    // the first of the order has not got the largest score when a bias or groups decide
-    const double l = !in ? 0.0 : a.r.sigmoid ? log_sigmoid(chosen) : (double)chosen;
-    double most = in ? l : -__builtin_inf();
-    for (uint32_t m = 1; m < slots; m *= 2) most = fmax(most, __shfl_xor(most, (int)m, 64));
-    w = in ? exp(l - most) : 0.0;
+    // relative to the largest of the chosen, which need not be the first of the order: a bias or groups may have decided
+    float top = in ? (a.r.sigmoid ? fminf(chosen, 0.0f) : chosen) : -__builtin_inff();
+    for (uint32_t m = 1; m < slots; m *= 2) top = fmaxf(top, __shfl_xor(top, (int)m, 64));
+    if (in) w = a.r.sigmoid ? sigmoid_over(chosen, top) : exp_negative((double)chosen - (double)top);
     double all = w;
     for (uint32_t m = 1; m < slots; m *= 2) all += __shfl_xor(all, (int)m, 64);
     w = all > 0.0 ? w / all : 0.0;
   } else if (in) {
-    w = a.r.sigmoid ? 1.0 / (1.0 + exp(-(double)chosen)) : exp((double)chosen - (double)zmax) / sum;
+    w = a.r.sigmoid ? sigmoid_over(chosen, 0.0) : exp_negative((double)chosen - (double)zmax) / sum;
   }
   if (mine) {
     a.ids[(uint64_t)row * k + j] = id;
@@ -207,32 +223,20 @@ __device__ __forceinline__ float sum16(float v) {
   return v + __uint_as_float(turn16<1>(__float_as_uint(v)));
 }
 __device__ __forceinline__ uint32_t prefix16(uint32_t v) { return group_scan_u32<16>(v); }
-// How many of the 16 lanes hold more; with `or_equal_before`, equal ones of smaller lanes too.
-template <int N = 1>
-__device__ __forceinline__ uint32_t larger16(uint32_t v, uint32_t sub, bool or_equal_before) {
+// How many of the 16 lanes hold more; EQUAL: or as much and are smaller.
+template <bool EQUAL, int N = 1>
+__device__ __forceinline__ uint32_t larger16(uint32_t v, uint32_t sub) {
   const uint32_t o = turn16<N>(v);
-  const uint32_t mine = o > v || (or_equal_before && o == v && sub >= N);  // lane (l - N) mod 16 is smaller than l where l >= N
+  const uint32_t mine = EQUAL ? o > v || (o == v && sub >= N) : o > v;  // lane (l - N) mod 16 is smaller than l where l >= N
   if constexpr (N < 15)
-    return mine + larger16<N + 1>(v, sub, or_equal_before);
+    return mine + larger16<EQUAL, N + 1>(v, sub);
   else
     return mine;
 }
-// e^x of x <= 0, to some 1e-14
-__device__ __forceinline__ double exp_negative(double x) {
-  const double t = fmax(x * 1.44269504088896340736, -1000.0), n = rint(t), f = (t - n) * 0.69314718055994530942;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, f, 1.0 / 3628800.0);
-  p = fma(p, f, 1.0 / 362880.0);
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
-  p = fma(p, f, 1.0);
-  return __longlong_as_double(__double_as_longlong(p) + ((long long)(int)n << 52));
+// The same row's lane across: N = 1, 2, 4, 8 (4 and 8: of values that are the same in all of the 4 or 8 lanes that mirror one another)
+template <int N>
+__device__ __forceinline__ uint32_t across(uint32_t v) {
+  return dpp0<N == 1 ? DPP_QUAD_XOR1 : N == 2 ? DPP_QUAD_XOR2 : N == 4 ? DPP_ROW_HALF_MIRROR : DPP_ROW_MIRROR, 0xF>(v);
 }
 
 template <typename T, int PER>
@@ -244,10 +248,12 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
     for (uint32_t e = threadIdx.x; e < E; e += 64 * ROUTE_WAVES) a.counts[e] = 0;
   struct Wave {
     union {
-      uint32_t key[4][16 * PER];  // of the four rows, where groups are not whole lanes
       struct {
+        uint32_t key[4][16 * PER];         // of the four rows
         float listed[4][QUAD_LISTED + 4];  // choices (logits where it goes by them), filled up to four with what is none
         uint32_t expert[4][QUAD_LISTED];
+        float best[4][QUAD_K + 2];  // the k best and the one after them
+        uint32_t place[4][QUAD_K + 2];
       };
       double exact[64 * WIDE];
     };
@@ -312,7 +318,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
       float c[PER], most = 1.0f;
       if (a.r.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) c[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fminf(-z[i] * 1.44269504f, 126.0f)));
+        for (int i = 0; i < PER; ++i) c[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[i] * -1.44269504f));  // of a closed one: 0
       } else {
         float sum = 0.0f;
 #pragma unroll
@@ -342,11 +348,14 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
           second = max(second, min(best, key[i]));
           best = max(best, key[i]);
         }
-        for (uint32_t m = 1; m < lanes; m *= 2) {
-          const uint32_t b = (uint32_t)__shfl_xor((int)best, (int)m, 64), c = (uint32_t)__shfl_xor((int)second, (int)m, 64);
+        auto join = [&](uint32_t b, uint32_t c) {
           second = max(min(best, b), max(second, c));
           best = max(best, b);
-        }
+        };
+        if (lanes > 1) join(across<1>(best), across<1>(second));
+        if (lanes > 2) join(across<2>(best), across<2>(second));
+        if (lanes > 4) join(across<4>(best), across<4>(second));
+        if (lanes > 8) join(across<8>(best), across<8>(second));
         owner = sub & ~(lanes - 1);
       } else {
 #pragma unroll
@@ -364,7 +373,8 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
       uint32_t mine = best;
       if (best && second && a.r.group_top2) mine = score_key(key_score(best) + key_score(second));
       if (owner != sub) mine = 0;
-      const bool stays = mine && larger16(mine, sub, true) < a.r.groups_kept;
+      bool stays = mine && larger16<false>(mine, sub) < a.r.groups_kept;
+      if (__ballot((uint32_t)__popc((uint32_t)(__ballot(stays) >> (lane & 48)) & 0xFFFFu) > a.r.groups_kept)) stays = mine && larger16<true>(mine, sub) < a.r.groups_kept;  // equal ones
       const uint32_t last = min16(stays ? mine : 0xFFFFFFFFu), next = max16(stays ? 0 : mine);
       if (!by_logit && next) doubt = !(key_score(last) - key_score(next) > 3.0f * near);
       const uint32_t stay = (uint32_t)(__ballot(stays) >> (lane & 48)) & 0xFFFFu;
@@ -384,50 +394,50 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
     uint32_t top = key[0];
 #pragma unroll
     for (int i = 1; i < PER; ++i) top = max(top, key[i]);
-    uint32_t least = min16(larger16(top, sub, false) < k ? top : 0xFFFFFFFFu);
+    uint32_t least = min16(larger16<false>(top, sub) < k ? top : 0xFFFFFFFFu);
     if (!by_logit && least) least = score_key(key_score(least) - near);
     least = max(least, 1u);
-    uint32_t mine = 0;
+    uint32_t wanted = 0;  // bits of the lane's candidates
 #pragma unroll
-    for (int i = 0; i < PER; ++i) mine += key[i] >= least;
-    const uint32_t sum = prefix16(mine), count = (uint32_t)__shfl((int)sum, (int)(lane | 15), 64);
+    for (int i = 0; i < PER; ++i) wanted |= key[i] >= least ? 1u << i : 0u;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s.key[quarter][sub * PER + i] = key[i];
+    const uint32_t mine = (uint32_t)__popc(wanted), sum = prefix16(mine);
+    const uint32_t count = (uint32_t)__shfl((int)sum, (int)(lane | 15), 64), listed = min(count, QUAD_LISTED);
     if (count > QUAD_LISTED) doubt = true;
-    uint32_t at = sum - mine;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (key[i] >= least) {
-        if (at < QUAD_LISTED) {
-          s.listed[quarter][at] = key_score(key[i]);
-          s.expert[quarter][at] = sub * PER + i;
-        }
-        ++at;
-      }
-    const uint32_t listed = min(count, QUAD_LISTED);
+    __builtin_amdgcn_wave_barrier();
+    for (uint32_t at = sum - mine; wanted && at < QUAD_LISTED; ++at) {
+      const uint32_t e = sub * PER + (uint32_t)__builtin_ctz(wanted);
+      wanted &= wanted - 1;
+      s.listed[quarter][at] = key_score(s.key[quarter][e]);
+      s.expert[quarter][at] = e;
+    }
     if (sub < 4) s.listed[quarter][listed + sub] = -__builtin_inff();
+    if (sub == 0 && listed <= k) s.best[quarter][listed] = -__builtin_inff();
     __builtin_amdgcn_wave_barrier();
     for (uint32_t c = sub; c < listed; c += 16) {
+      // candidates stand by number: of equal ones the first comes first
       const float v = s.listed[quarter][c];
-      uint32_t rank = 0, close = 0;
+      const uint32_t e = s.expert[quarter][c];
+      uint32_t rank = 0;
       for (uint32_t j = 0; j < listed; j += 4) {
         const float4 o = *(const float4*)&s.listed[quarter][j];
-        const float four[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          rank += four[i] > v || (four[i] == v && j + i < c);
-          close += fabsf(four[i] - v) <= near;  // itself among them
-        }
+        rank += o.x > v || (o.x == v && j < c);
+        rank += o.y > v || (o.y == v && j + 1 < c);
+        rank += o.z > v || (o.z == v && j + 2 < c);
+        rank += o.w > v || (o.w == v && j + 3 < c);
       }
-      const uint32_t e = s.expert[quarter][c];
-      if (rank < k) {
-        if (!by_logit && close > 1)
-          for (uint32_t j = 0; j < listed; ++j)
-            if (fabsf(s.listed[quarter][j] - v) <= near) {
-              // alike, the same logit and bias, they stand as they are
-              const uint32_t f = s.expert[quarter][j];
-              doubt |= !((float)x[e] == (float)x[f] && (!a.r.bias || a.r.bias[e] == a.r.bias[f]));
-            }
-        if (n < rows) s.id[n * slots + rank] = e;
+      if (rank <= k) {
+        s.best[quarter][rank] = v;
+        s.place[quarter][rank] = e;
+        if (rank < k && n < rows) s.id[n * slots + rank] = e;
       }
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (!by_logit && sub < k && sub < listed && !(s.best[quarter][sub] - s.best[quarter][sub + 1] > near)) {
+      // alike, the same logit and bias, they stand as they are
+      const uint32_t e = s.place[quarter][sub], f = s.place[quarter][sub + 1];
+      doubt |= !((float)x[e] == (float)x[f] && (!a.r.bias || a.r.bias[e] == a.r.bias[f]));
     }
     // rows in doubt, one after another by the whole wavefront
     uint64_t rest = __ballot(doubt);
@@ -489,7 +499,10 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
     if (full_sum) {
       double sum = 0.0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) sum += open_expert(z[i]) ? exp((double)z[i] - (double)zmax) : 0.0;
+      for (int i = 0; i < PER; ++i) {
+        const double w = exp_negative((double)z[i] - (double)zmax);
+        sum += open_expert(z[i]) ? w : 0.0;
+      }
       sum = group_sum_f64<64>(sum);
       if (lane / slots == n) {
         my_sum = sum;
