@@ -4,10 +4,18 @@
 //   y = y - (presence + frequency * n(t))      if n(t) > 0
 //   y = y + bias(t)
 //   y = -inf                                   if a mask or the graph's row does not allow t
-// One pass: every logit is read once and written once, by the same thread, so that a call may work in place.  A workgroup has a
-// tile of a row, 16 columns a thread, and turns the sparse parts (history, biases, neighbours) into arrays over the tile's
-// columns in LDS: counts by integer atomics, whose order does not matter, biases by the thread that meets the first of
-// equal ids.  All of a row's tiles read its whole history, from L2.
+// One pass: every logit is read once at most and written once, before anything overwrites it, so that a call may work in place.
+//
+// adjust_kernel: a workgroup has a tile of a row, 16 columns a thread, and turns the sparse parts (history, biases, neighbours) into
+// arrays over the tile's columns in LDS: counts by integer atomics, whose order does not matter, biases by the thread that
+// meets the first of equal ids.  All of a row's tiles read its whole history, from L2.
+//
+// adjust_near_kernel: rows that a graph holds to a vertex's neighbours, up to NEAR of them.  A workgroup has a row: the neighbours
+// go into a hash table in LDS, where history and biases look themselves up, their logits into registers; the row is filled with
+// -inf by a stream of stores, and the neighbours are put in.  Nothing else of the logits is read.  (4,096 rows of 65,536 f16:
+// tiles 234 us, most of it the wait for state, row bounds and neighbours, eight
+// times a row; so 110.)  Rows with more neighbours
+// are done tile by tile by their workgroup.
 #include "sky_graph.h"
 #include "sky_scores.h"
 
@@ -40,12 +48,63 @@ __device__ __forceinline__ uint32_t lower_bound(const uint32_t* a, uint32_t lo, 
   return lo;
 }
 
+// The history of a row: f(id, counted) for each.  Eight loads at a time.
+template <typename F>
+__device__ __forceinline__ void each_of_history(const AdjustArgs& a, uint32_t row, F f) {
+  const uint32_t n = a.r.history_lengths ? min(a.r.history_lengths[row], a.r.history_columns) : a.r.history_columns;
+  const uint32_t from = a.r.history_first ? a.r.history_first[row] : 0u;
+  const uint32_t* const h = a.r.history + row * a.r.history_stride;
+  for (uint32_t base = threadIdx.x; base < n; base += 8 * blockDim.x) {
+    uint32_t id[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) id[i] = base + i * blockDim.x < n ? h[base + i * blockDim.x] : SKY_INVALID;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+      if (id[i] < a.columns) f(id[i], base + i * blockDim.x >= from);
+  }
+}
+// The biases of a row between two columns: f(id, sum of its values) for each id.
+template <typename F>
+__device__ __forceinline__ void each_bias(const AdjustArgs& a, uint32_t row, uint32_t lowest, uint32_t end_column, F f) {
+  const uint32_t begin = min(a.r.bias_offsets[row], a.r.bias_count), end = min(a.r.bias_offsets[row + 1], a.r.bias_count);
+  uint32_t lo = begin, hi = end;
+  if (hi > lo && hi - lo > BIAS_SEARCH_MIN) {
+    lo = lower_bound(a.r.bias_ids, lo, hi, lowest);
+    hi = lower_bound(a.r.bias_ids, lo, hi, end_column);
+  }
+  for (uint32_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+    const uint32_t id = a.r.bias_ids[i];
+    if (id < a.columns && (i == begin || a.r.bias_ids[i - 1] != id)) {
+      float sum = a.r.bias_values[i];
+      for (uint32_t j = i + 1; j < end && a.r.bias_ids[j] == id; ++j) sum += a.r.bias_values[j];
+      f(id, sum);
+    }
+  }
+}
+// What becomes of a logit that is allowed.
+struct Change {
+  float rep, presence, frequency;
+  __device__ __forceinline__ Change(const AdjustArgs& a, uint32_t row) {
+    const bool history = a.r.history != nullptr;
+    rep = history && a.r.repetition ? a.r.repetition[row] : 1.0f;
+    presence = history && a.r.presence ? a.r.presence[row] : 0.0f;
+    frequency = history && a.r.frequency ? a.r.frequency[row] : 0.0f;
+  }
+  // n: how often it was counted, and SEEN
+  __device__ __forceinline__ float of(float s, uint32_t n) const {
+    if (n) {
+      s = s > 0.0f ? s / rep : s * rep;
+      if (n & ~SEEN) s -= presence + frequency * (float)(n & ~SEEN);
+    }
+    return s;
+  }
+};
+
+// Tile t of a row, by the workgroup; `lds` holds what tile_words says.
 template <typename T>
-__global__ __launch_bounds__(512) void adjust_kernel(AdjustArgs a) {
+__device__ __forceinline__ void adjust_tile(const AdjustArgs& a, uint32_t row, uint32_t t, uint32_t* lds) {
   constexpr int N = Piece<T>::N, NV = COLS / N;
-  extern __shared__ uint32_t lds[];
   const uint32_t threads = blockDim.x, tid = threadIdx.x, tile = COLS * threads;
-  const uint32_t row = blockIdx.x / a.tiles, t = blockIdx.x % a.tiles;
   const T* const x = (const T*)a.logits + row * a.stride;
   T* const y = (T*)a.out + row * a.out_stride;
   // tiles begin where stores are aligned
@@ -74,7 +133,7 @@ __global__ __launch_bounds__(512) void adjust_kernel(AdjustArgs a) {
         if (c + e >= 0 && c + e < columns) v[i].e[e] = x[c + e];
     }
   };
-  const bool early = !masked && !graph && !none;  // all of the row is needed: its loads run beside the scans below
+  const bool early = !graph && !none;  // the row is needed (a mask leaves something of most pieces): its loads run beside the scans below
   if (early) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) load(i);
@@ -87,36 +146,20 @@ __global__ __launch_bounds__(512) void adjust_kernel(AdjustArgs a) {
   if (words && !none) {
     for (uint32_t i = tid; i < words / 4; i += threads) ((uint4*)lds)[i] = uint4{0, 0, 0, 0};
     __syncthreads();
-    if (history) {
-      const uint32_t n = a.r.history_lengths ? min(a.r.history_lengths[row], a.r.history_columns) : a.r.history_columns;
-      const uint32_t from = a.r.history_first ? a.r.history_first[row] : 0u;
-      const uint32_t* const h = a.r.history + row * a.r.history_stride;
-      for (uint32_t i = tid; i < n; i += threads) {
-        const uint32_t id = h[i], at = id - c0;
-        if (at < tile && id < a.columns) {
-          if (i >= from)
+    if (history)
+      each_of_history(a, row, [&](uint32_t id, bool counted) {
+        const uint32_t at = id - c0;
+        if (at < tile) {
+          if (counted)
             atomicAdd(&count[at], 1u);
           else
             atomicOr(&count[at], SEEN);
         }
-      }
-    }
-    if (biased) {
-      uint32_t lo = min(a.r.bias_offsets[row], a.r.bias_count), hi = min(a.r.bias_offsets[row + 1], a.r.bias_count);
-      const uint32_t begin = lo, end = hi;
-      if (hi > lo && hi - lo > BIAS_SEARCH_MIN) {
-        lo = lower_bound(a.r.bias_ids, lo, hi, (uint32_t)max(first, 0));
-        hi = lower_bound(a.r.bias_ids, lo, hi, (uint32_t)min((int64_t)first + tile, (int64_t)columns));
-      }
-      for (uint32_t i = lo + tid; i < hi; i += threads) {
-        const uint32_t id = a.r.bias_ids[i], at = id - c0;
-        if (at < tile && id < a.columns && (i == begin || a.r.bias_ids[i - 1] != id)) {
-          float sum = a.r.bias_values[i];
-          for (uint32_t j = i + 1; j < end && a.r.bias_ids[j] == id; ++j) sum += a.r.bias_values[j];
-          bias[at] = sum;
-        }
-      }
-    }
+      });
+    if (biased)
+      each_bias(a, row, (uint32_t)max(first, 0), (uint32_t)min((int64_t)first + tile, (int64_t)columns), [&](uint32_t id, float sum) {
+        if (id - c0 < tile) bias[id - c0] = sum;
+      });
     if (graph) {
       const uint32_t s = a.r.states[row * a.r.states_stride];
       if (s < a.V) {
@@ -129,9 +172,7 @@ __global__ __launch_bounds__(512) void adjust_kernel(AdjustArgs a) {
     }
     __syncthreads();
   }
-  const float rep = history && a.r.repetition ? a.r.repetition[row] : 1.0f;
-  const float presence = history && a.r.presence ? a.r.presence[row] : 0.0f;
-  const float frequency = history && a.r.frequency ? a.r.frequency[row] : 0.0f;
+  const Change change(a, row);
 
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -158,13 +199,7 @@ __global__ __launch_bounds__(512) void adjust_kernel(AdjustArgs a) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       float s = (float)v[i].e[e];
-      if (history) {
-        const uint32_t n = count[at + e];
-        if (n) {
-          s = s > 0.0f ? s / rep : s * rep;
-          if (n & ~SEEN) s -= presence + frequency * (float)(n & ~SEEN);
-        }
-      }
+      if (history) s = change.of(s, count[at + e]);
       if (biased) s += bias[at + e];
       o.e[e] = (T)(stay >> e & 1u ? s : -__builtin_inff());
     }
@@ -176,6 +211,131 @@ __global__ __launch_bounds__(512) void adjust_kernel(AdjustArgs a) {
         if (c + e >= 0 && c + e < columns) y[c + e] = o.e[e];
     }
   }
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void adjust_kernel(AdjustArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+  adjust_tile<T>(a, blockIdx.x / a.tiles, blockIdx.x % a.tiles, lds);
+}
+
+constexpr uint32_t NEAR_THREADS = 256, NEAR = 1024, SLOTS = 2 * NEAR;  // the table is half full at most
+template <typename T>
+__global__ __launch_bounds__(NEAR_THREADS) void adjust_near_kernel(AdjustArgs a) {
+  constexpr uint32_t N = Piece<T>::N, EACH = NEAR / NEAR_THREADS;
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];  // key, count and bias of a slot, or what a tile takes
+  uint32_t* const key = lds;
+  uint32_t* const count = lds + SLOTS;
+  float* const bias = (float*)(lds + 2 * SLOTS);
+  const uint32_t tid = threadIdx.x, row = blockIdx.x;
+  const T* const x = (const T*)a.logits + row * a.stride;
+  T* const y = (T*)a.out + row * a.out_stride;
+  const uint32_t state = a.r.states[row * a.r.states_stride];
+  uint32_t lo = 0, hi = 0;
+  if (state < a.V) {
+    lo = a.xadj[state];
+    hi = a.xadj[state + 1];
+  }
+  if (hi - lo > NEAR) {
+    for (uint32_t t = 0; t < a.tiles; ++t) {
+      adjust_tile<T>(a, row, t, lds);
+      __syncthreads();
+    }
+    return;
+  }
+  const uint32_t* mask = nullptr;
+  if (a.r.allowed) {
+    const uint32_t m = a.r.allowed_row ? a.r.allowed_row[row] : a.r.allowed_rows == 1 ? 0u : row;
+    if (m != SKY_INVALID) {
+      if (m >= a.r.allowed_rows)
+        hi = lo;  // nothing
+      else
+        mask = a.r.allowed + m * a.r.allowed_stride;
+    }
+  }
+  const bool tables = a.r.history || a.r.bias_ids;
+  uint32_t id[EACH], slot[EACH];
+  float value[EACH];
+#pragma unroll
+  for (uint32_t i = 0; i < EACH; ++i) {
+    const uint32_t j = lo + tid + i * NEAR_THREADS;
+    id[i] = j < hi ? a.adjncy[j] : SKY_INVALID;
+    if (id[i] >= a.columns || (mask && !(mask[id[i] >> 5] >> (id[i] & 31) & 1u))) id[i] = SKY_INVALID;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < EACH; ++i) value[i] = id[i] != SKY_INVALID ? (float)x[id[i]] : 0.0f;
+  if (tables) {
+    auto first_slot = [](uint32_t v) { return (v * 0x9E3779B1u) >> 21; };
+    static_assert(SLOTS == 1u << 11, "of 11 bits");
+    for (uint32_t i = tid; i < SLOTS; i += NEAR_THREADS) {
+      key[i] = SKY_INVALID;
+      count[i] = 0;
+      bias[i] = 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i)
+      if (id[i] != SKY_INVALID) {
+        uint32_t s = first_slot(id[i]);
+        for (;;) {
+          const uint32_t was = atomicCAS(&key[s], SKY_INVALID, id[i]);
+          if (was == SKY_INVALID || was == id[i]) break;
+          s = (s + 1) & (SLOTS - 1);
+        }
+        slot[i] = s;
+      }
+    __syncthreads();
+    auto find = [&](uint32_t v) {  // its slot; one without its key: it is none of the neighbours
+      uint32_t s = first_slot(v);
+      while (key[s] != v && key[s] != SKY_INVALID) s = (s + 1) & (SLOTS - 1);
+      return s;
+    };
+    if (a.r.history)
+      each_of_history(a, row, [&](uint32_t v, bool counted) {
+        const uint32_t s = find(v);
+        if (key[s] == v) {
+          if (counted)
+            atomicAdd(&count[s], 1u);
+          else
+            atomicOr(&count[s], SEEN);
+        }
+      });
+    if (a.r.bias_ids)
+      each_bias(a, row, 0, a.columns, [&](uint32_t v, float sum) {
+        const uint32_t s = find(v);
+        if (key[s] == v) bias[s] = sum;
+      });
+  }
+  auto settled = [] {  // what this thread has loaded and stored is done, and every thread's is
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __syncthreads();
+  };
+  settled();  // no store before every neighbour's logit is here: the call may work in place
+  // the row without its neighbours: whole pieces where stores are aligned, elements before and after
+  const T gone = (T)-__builtin_inff();
+  Piece<T> none;
+#pragma unroll
+  for (uint32_t e = 0; e < N; ++e) none.e[e] = gone;
+  const uint32_t head = min((uint32_t)((16 - (uintptr_t)y % 16) % 16 / sizeof(T)), a.columns), pieces = (a.columns - head) / N;
+  // Every row from a place of its own: rows of a power of two apart would all be at the same channel of memory at a time (4,096 rows
+  // of 128 KB 325 us instead of 110).
+  const uint32_t shift = (uint32_t)((uint64_t)pieces * (row * 0x9E3779B1u) >> 32) & ~(NEAR_THREADS - 1);
+  for (uint32_t i = tid; i < pieces; i += NEAR_THREADS) {
+    const uint32_t p = i + shift;
+    store_piece(y + head + (p < pieces ? p : p - pieces) * N, none);
+  }
+  if (tid < head) y[tid] = gone;
+  if (head + pieces * N + tid < a.columns) y[head + pieces * N + tid] = gone;
+  settled();  // the neighbours' stores come after those; counts and biases are whole
+  const Change change(a, row);
+#pragma unroll
+  for (uint32_t i = 0; i < EACH; ++i)
+    if (id[i] != SKY_INVALID) {
+      float v = value[i];
+      if (a.r.history) v = change.of(v, count[slot[i]]);
+      if (a.r.bias_ids) v += bias[slot[i]];
+      y[id[i]] = (T)v;
+    }
 }
 
 int check_rules(const sky_logits_rules* r, uint32_t rows, uint32_t columns, AdjustArgs* a) {
@@ -258,18 +418,32 @@ extern "C" int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, u
   a.stride = row_stride;
   a.out_stride = out_stride;
   a.columns = columns;
+  const size_t size = dtype_size(dtype);
+  const bool aligned = ((uintptr_t)out | out_stride * size) % 16 == 0;
+  const hipStream_t st = (hipStream_t)stream;
+  auto tiles = [&](uint32_t tile) { return (uint32_t)(((uint64_t)columns + (aligned ? 0 : 16 / size - 1) + tile - 1) / tile); };
+  if (a.xadj) {
+    const uint32_t tile = NEAR_THREADS * COLS;
+    a.tiles = tiles(tile);
+    const bool tables = a.r.history || a.r.bias_ids;
+    const size_t lds = std::max<size_t>(tables ? 3 * SLOTS : 0, (a.r.history ? tile : 0u) + (a.r.bias_ids ? tile : 0u) + tile / 32) * 4;
+    if (dtype == SKY_F32)
+      hipLaunchKernelGGL(adjust_near_kernel<float>, dim3(rows), dim3(NEAR_THREADS), lds, st, a);
+    else if (dtype == SKY_F16)
+      hipLaunchKernelGGL(adjust_near_kernel<_Float16>, dim3(rows), dim3(NEAR_THREADS), lds, st, a);
+    else
+      hipLaunchKernelGGL(adjust_near_kernel<__bf16>, dim3(rows), dim3(NEAR_THREADS), lds, st, a);
+    return check_launch();
+  }
   // counts and biases take 8 bytes of LDS a column: half the tile keeps several workgroups on a CU
   const uint32_t most = a.r.history && a.r.bias_ids ? 256 : 512;
   uint32_t threads = 64;
   while (threads < most && threads * COLS < columns) threads *= 2;
   const uint32_t tile = threads * COLS;
-  const size_t size = dtype_size(dtype);
-  const bool aligned = ((uintptr_t)out | out_stride * size) % 16 == 0;
-  a.tiles = (uint32_t)(((uint64_t)columns + (aligned ? 0 : 16 / size - 1) + tile - 1) / tile);
+  a.tiles = tiles(tile);
   if ((uint64_t)a.tiles * rows > 0x7FFFFFFFull) return fail(SKY_ERR_LIMIT, "sky_logits_adjust: too many tiles");
-  const size_t lds = ((a.r.history ? tile : 0u) + (a.r.bias_ids ? tile : 0u) + (a.xadj ? tile / 32 : 0u)) * 4;
+  const size_t lds = ((a.r.history ? tile : 0u) + (a.r.bias_ids ? tile : 0u)) * 4;
   const dim3 grid(a.tiles * rows), block(threads);
-  const hipStream_t st = (hipStream_t)stream;
   if (dtype == SKY_F32)
     hipLaunchKernelGGL(adjust_kernel<float>, grid, block, lds, st, a);
   else if (dtype == SKY_F16)
