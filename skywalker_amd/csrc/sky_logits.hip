@@ -48,11 +48,20 @@ __device__ __forceinline__ uint32_t lower_bound(const uint32_t* a, uint32_t lo, 
   return lo;
 }
 
+// Where a row's history and biases lie: asked for before anything that waits.
+struct Sparse {
+  uint32_t n, from, begin, end;
+  __device__ __forceinline__ Sparse(const AdjustArgs& a, uint32_t row) {
+    n = !a.r.history ? 0 : a.r.history_lengths ? min(a.r.history_lengths[row], a.r.history_columns) : a.r.history_columns;
+    from = a.r.history_first ? a.r.history_first[row] : 0u;
+    begin = a.r.bias_ids ? min(a.r.bias_offsets[row], a.r.bias_count) : 0;
+    end = a.r.bias_ids ? min(a.r.bias_offsets[row + 1], a.r.bias_count) : 0;
+  }
+};
 // The history of a row: f(id, counted) for each.  Eight loads at a time.
 template <typename F>
-__device__ __forceinline__ void each_of_history(const AdjustArgs& a, uint32_t row, F f) {
-  const uint32_t n = a.r.history_lengths ? min(a.r.history_lengths[row], a.r.history_columns) : a.r.history_columns;
-  const uint32_t from = a.r.history_first ? a.r.history_first[row] : 0u;
+__device__ __forceinline__ void each_of_history(const AdjustArgs& a, uint32_t row, const Sparse& p, F f) {
+  const uint32_t n = p.n, from = p.from;
   const uint32_t* const h = a.r.history + row * a.r.history_stride;
   for (uint32_t base = threadIdx.x; base < n; base += 8 * blockDim.x) {
     uint32_t id[8];
@@ -65,8 +74,8 @@ __device__ __forceinline__ void each_of_history(const AdjustArgs& a, uint32_t ro
 }
 // The biases of a row between two columns: f(id, sum of its values) for each id.
 template <typename F>
-__device__ __forceinline__ void each_bias(const AdjustArgs& a, uint32_t row, uint32_t lowest, uint32_t end_column, F f) {
-  const uint32_t begin = min(a.r.bias_offsets[row], a.r.bias_count), end = min(a.r.bias_offsets[row + 1], a.r.bias_count);
+__device__ __forceinline__ void each_bias(const AdjustArgs& a, const Sparse& p, uint32_t lowest, uint32_t end_column, F f) {
+  const uint32_t begin = p.begin, end = p.end;
   uint32_t lo = begin, hi = end;
   if (hi > lo && hi - lo > BIAS_SEARCH_MIN) {
     lo = lower_bound(a.r.bias_ids, lo, hi, lowest);
@@ -120,23 +129,38 @@ __device__ __forceinline__ void adjust_tile(const AdjustArgs& a, uint32_t row, u
   }
   const bool masked = mask_row != SKY_INVALID && !none;
   const bool whole_tile = first >= 0 && first + (int)tile <= columns;
+  const Sparse sparse(a, row);
+  const Change change(a, row);
 
   Piece<T> v[NV];
+  uint32_t stay[NV];  // bits of the elements that masks leave
   auto column = [&](int i) { return first + (int)((i * threads + tid) * N); };
-  auto load = [&](int i) {
-    const int c = column(i);
-    if (whole_tile || (c >= 0 && c + N <= columns)) {
-      v[i] = load_piece(x + c);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (c + e >= 0 && c + e < columns) v[i].e[e] = x[c + e];
-    }
+  auto whole = [&](int c) { return whole_tile || (c >= 0 && c + N <= columns); };
+  auto load = [&](int i) {  // pieces that are not whole are read element by element
+    if (whole(column(i))) v[i] = load_piece(x + column(i));
   };
   const bool early = !graph && !none;  // the row is needed (a mask leaves something of most pieces): its loads run beside the scans below
   if (early) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) load(i);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = column(i);
+    stay[i] = none ? 0u : (1u << N) - 1;
+    if (masked) {
+      const uint32_t* const m = a.r.allowed + mask_row * a.r.allowed_stride;
+      if (whole(c)) {
+        const uint64_t lo = m[(uint32_t)c >> 5], hi = m[(uint32_t)(c + N - 1) >> 5];
+        stay[i] &= (uint32_t)((lo | hi << 32) >> (c & 31));
+      } else {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (c + e >= 0 && c + e < columns) bits |= (m[(uint32_t)(c + e) >> 5] >> ((c + e) & 31) & 1u) << e;
+        stay[i] &= bits;
+      }
+    }
   }
 
   uint32_t* const count = lds;
@@ -147,7 +171,7 @@ __device__ __forceinline__ void adjust_tile(const AdjustArgs& a, uint32_t row, u
     for (uint32_t i = tid; i < words / 4; i += threads) ((uint4*)lds)[i] = uint4{0, 0, 0, 0};
     __syncthreads();
     if (history)
-      each_of_history(a, row, [&](uint32_t id, bool counted) {
+      each_of_history(a, row, sparse, [&](uint32_t id, bool counted) {
         const uint32_t at = id - c0;
         if (at < tile) {
           if (counted)
@@ -157,7 +181,7 @@ __device__ __forceinline__ void adjust_tile(const AdjustArgs& a, uint32_t row, u
         }
       });
     if (biased)
-      each_bias(a, row, (uint32_t)max(first, 0), (uint32_t)min((int64_t)first + tile, (int64_t)columns), [&](uint32_t id, float sum) {
+      each_bias(a, sparse, (uint32_t)max(first, 0), (uint32_t)min((int64_t)first + tile, (int64_t)columns), [&](uint32_t id, float sum) {
         if (id - c0 < tile) bias[id - c0] = sum;
       });
     if (graph) {
@@ -172,43 +196,45 @@ __device__ __forceinline__ void adjust_tile(const AdjustArgs& a, uint32_t row, u
     }
     __syncthreads();
   }
-  const Change change(a, row);
 
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = column(i);
     const uint32_t at = (i * threads + tid) * N;
-    const bool whole = whole_tile || (c >= 0 && c + N <= columns);
-    uint32_t stay = none ? 0u : (1u << N) - 1;
-    if (masked) {
-      const uint32_t* const m = a.r.allowed + mask_row * a.r.allowed_stride;
-      if (whole) {
-        const uint64_t lo = m[(uint32_t)c >> 5], hi = m[(uint32_t)(c + N - 1) >> 5];
-        stay &= (uint32_t)((lo | hi << 32) >> (c & 31));
-      } else {
-        uint32_t bits = 0;
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (c + e >= 0 && c + e < columns) bits |= (m[(uint32_t)(c + e) >> 5] >> ((c + e) & 31) & 1u) << e;
-        stay &= bits;
-      }
-    }
-    if (graph && !none) stay &= can[at >> 5] >> (at & 31);  // N divides 32: the piece's bits lie in one word
-    if (!early && stay) load(i);
-    Piece<T> o;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      float s = (float)v[i].e[e];
+    if (graph && !none) stay[i] &= can[at >> 5] >> (at & 31);  // N divides 32: the piece's bits lie in one word
+    if (!early && stay[i]) load(i);
+    auto adjusted = [&](T logit, uint32_t e) {
+      float s = (float)logit;
       if (history) s = change.of(s, count[at + e]);
       if (biased) s += bias[at + e];
-      o.e[e] = (T)(stay >> e & 1u ? s : -__builtin_inff());
-    }
-    if (whole) {
+      return (T)(stay[i] >> e & 1u ? s : -__builtin_inff());
+    };
+    if (whole(c)) {
+      Piece<T> o;
+      float s[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[e] = (float)v[i].e[e];
+      if (history) {
+        uint32_t n[N], any = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) any |= n[e] = count[at + e];
+        if (any)  // of most pieces nothing was visited
+#pragma unroll
+          for (int e = 0; e < N; ++e) s[e] = change.of(s[e], n[e]);
+      }
+      if (biased)
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] += bias[at + e];
+      if (__builtin_expect(stay[i] != (1u << N) - 1, 1))
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] = stay[i] >> e & 1u ? s[e] : -__builtin_inff();
+#pragma unroll
+      for (int e = 0; e < N; ++e) o.e[e] = (T)s[e];
       store_piece(y + c, o);
     } else {
-#pragma unroll
+#pragma unroll 1
       for (int e = 0; e < N; ++e)
-        if (c + e >= 0 && c + e < columns) y[c + e] = o.e[e];
+        if (c + e >= 0 && c + e < columns) y[c + e] = adjusted(x[c + e], e);
     }
   }
 }
@@ -254,6 +280,7 @@ __global__ __launch_bounds__(NEAR_THREADS) void adjust_near_kernel(AdjustArgs a)
     }
   }
   const bool tables = a.r.history || a.r.bias_ids;
+  const Sparse sparse(a, row);
   uint32_t id[EACH], slot[EACH];
   float value[EACH];
 #pragma unroll
@@ -291,7 +318,7 @@ __global__ __launch_bounds__(NEAR_THREADS) void adjust_near_kernel(AdjustArgs a)
       return s;
     };
     if (a.r.history)
-      each_of_history(a, row, [&](uint32_t v, bool counted) {
+      each_of_history(a, row, sparse, [&](uint32_t v, bool counted) {
         const uint32_t s = find(v);
         if (key[s] == v) {
           if (counted)
@@ -301,7 +328,7 @@ __global__ __launch_bounds__(NEAR_THREADS) void adjust_near_kernel(AdjustArgs a)
         }
       });
     if (a.r.bias_ids)
-      each_bias(a, row, 0, a.columns, [&](uint32_t v, float sum) {
+      each_bias(a, sparse, 0, a.columns, [&](uint32_t v, float sum) {
         const uint32_t s = find(v);
         if (key[s] == v) bias[s] = sum;
       });

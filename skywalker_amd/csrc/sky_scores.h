@@ -15,15 +15,17 @@ struct Piece {
   static constexpr int N = 16 / (int)sizeof(T);
   T e[N];
 };
+// (As words: of elements the compiler makes four loads.)
 template <typename T>
 __device__ __forceinline__ Piece<T> load_piece(const T* p) {
-  Piece<T> v;
-  __builtin_memcpy(&v, p, 16);
-  return v;
+  uint4 w;
+  __builtin_memcpy(&w, p, 16);
+  return __builtin_bit_cast(Piece<T>, w);
 }
 template <typename T>
 __device__ __forceinline__ void store_piece(T* p, const Piece<T>& v) {
-  __builtin_memcpy(p, &v, 16);
+  const uint4 w = __builtin_bit_cast(uint4, v);
+  __builtin_memcpy(p, &w, 16);
 }
 
 // NaN and -inf are -inf (not there), +inf is the largest number, -0 is 0: what is left compares as the order of a row asks.
