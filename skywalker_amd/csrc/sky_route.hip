@@ -647,70 +647,138 @@ __global__ __launch_bounds__(COUNT_THREADS) void count_experts_kernel(const uint
     if (c[e]) atomicAdd(&counts[e], c[e]);
 }
 
-template <typename T, int PER>
+// The gradient: G lanes have a row, NP pieces of 16 bytes each, the pieces of a row one after another over the lanes.  The chosen
+// entries' own parts meet the row in LDS.  (A wavefront a row, the parts by 64 exchanges between lanes: 32,768 x 256 fp32 34 us.)
+template <int G>
+__device__ __forceinline__ float group_max_f32(float v) {
+  if constexpr (G == 16)
+    return key_score(max16(score_key(v)));
+  else
+    return wave_max_f32(v);
+}
+template <int G>
+__device__ __forceinline__ float group_sum_f32(float v) {
+  if constexpr (G == 16)
+    return sum16(v);
+  else
+    return wave_sum_f32(v);
+}
+template <typename T, int G, int NP>
 __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_backward_kernel(RouteArgs a) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t row = blockIdx.x * ROUTE_WAVES + wave, E = a.experts, k = a.r.k;
-  if (row >= a.rows) return;
+  constexpr int N = Piece<T>::N, ROWS = 64 / G, KP = (int)MAX_K / G > 1 ? (int)MAX_K / G : 1;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % G;
+  const uint32_t want = (blockIdx.x * ROUTE_WAVES + wave) * ROWS + lane / G, E = a.experts, k = a.r.k;
+  __shared__ __attribute__((aligned(16))) float parts[ROUTE_WAVES][ROWS][G * NP * N];
+  if ((blockIdx.x * ROUTE_WAVES + wave) * ROWS >= a.rows) return;
+  const uint32_t row = min(want, a.rows - 1);  // lanes of rows that are not there go along
   const T* const x = (const T*)a.logits + row * a.stride;
   T* const dx = (T*)a.dlogits + row * a.dstride;
-  uint32_t id = SKY_INVALID;
-  float g = 0.0f, xj = -__builtin_inff();
-  if (lane < k) {
-    id = a.ids_in[(uint64_t)row * k + lane];
-    if (id < E) {
-      g = a.dweights[(uint64_t)row * k + lane] * a.r.scale;
-      xj = plain_score((float)x[id]);
-    }
-    if (!open_expert(xj)) id = SKY_INVALID;
-  }
-  const bool in = id != SKY_INVALID;
-  if (!in) g = 0.0f;
-  float zmax = -__builtin_inff(), total = 0.0f;
-  float z[PER];
+  float* const part = parts[wave][lane / G];
   const bool dense = !a.r.sigmoid && !a.r.renormalise;
+  uint32_t id[KP];
+  float g[KP], xj[KP], d[KP];
+#pragma unroll
+  for (int i = 0; i < KP; ++i) {
+    const uint32_t j = sub + G * i;
+    id[i] = j < k ? a.ids_in[(uint64_t)row * k + j] : SKY_INVALID;
+    g[i] = id[i] < E ? a.dweights[(uint64_t)row * k + j] * a.r.scale : 0.0f;
+    xj[i] = id[i] < E ? plain_score((float)x[id[i]]) : -__builtin_inff();
+    if (!open_expert(xj[i])) {
+      id[i] = SKY_INVALID;
+      g[i] = 0.0f;
+    }
+  }
+  float z[NP][N];
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int e = 0; e < N; ++e) z[i][e] = 0.0f;
+  float zmax = -__builtin_inff(), total = 0.0f;
   if (dense) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const uint32_t e = 64 * i + lane;
-      z[i] = e < E ? plain_score((float)x[e]) : -__builtin_inff();
-      zmax = fmaxf(zmax, z[i]);
-    }
-    zmax = wave_max_f32(zmax);
+    for (int i = 0; i < NP; ++i) {
+      const uint32_t c = (i * G + sub) * N;
+      if (c + N <= E) {
+        const Piece<T> v = load_piece(x + c);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      z[i] = open_expert(z[i]) ? expf(z[i] - zmax) : 0.0f;
-      total += z[i];
+        for (int e = 0; e < N; ++e) z[i][e] = plain_score((float)v.e[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) z[i][e] = c + e < E ? plain_score((float)x[c + e]) : -__builtin_inff();
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) zmax = fmaxf(zmax, z[i][e]);
     }
-    total = wave_sum_f32(total);
+    zmax = group_max_f32<G>(zmax);
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        z[i][e] = open_expert(z[i][e]) ? __builtin_amdgcn_exp2f((z[i][e] - zmax) * 1.44269504f) : 0.0f;
+        total += z[i][e];
+      }
+    total = group_sum_f32<G>(total);
   }
-  // the gradient at the chosen entry of this lane (in the dense case: what is added to -s_e * sum g s)
-  float d = 0.0f, mean = 0.0f;
+  // the gradient at the chosen entries (in the dense case: what is added to -s_e * sum g s)
+  float mean = 0.0f;
   if (a.r.renormalise) {
-    const float l = !in ? -__builtin_inff() : a.r.sigmoid ? fminf(xj, 0.0f) - log1pf(expf(-fabsf(xj))) : xj;
-    const float most = wave_max_f32(l);
-    float p = in ? expf(l - most) : 0.0f;
-    const float all = wave_sum_f32(p);
-    p = all > 0.0f ? p / all : 0.0f;
-    mean = wave_sum_f32(g * p);
-    d = p * (g - mean);
-    if (a.r.sigmoid) d *= in ? 1.0f / (1.0f + expf(xj)) : 0.0f;
-  } else if (a.r.sigmoid) {
-    d = in ? g * (1.0f / (1.0f + expf(-xj))) * (1.0f / (1.0f + expf(xj))) : 0.0f;
-  } else {
-    d = in ? g * expf(xj - zmax) / total : 0.0f;
-    mean = wave_sum_f32(d);
-  }
+    // shares relative to the largest of the chosen: e^min(x, 0) / (1 + e^-|x|) is a sigmoid
+    float most = -__builtin_inff(), all = 0.0f;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const uint32_t e = 64 * i + lane;
-    float v = dense && total > 0.0f ? -(z[i] / total) * mean : 0.0f;
-    for (uint32_t j = 0; j < k; ++j) {
-      const uint32_t c = (uint32_t)__shfl((int)id, (int)j, 64);
-      const float add = __shfl(d, (int)j, 64);
-      if (c == e) v += add;
+    for (int i = 0; i < KP; ++i)
+      if (id[i] != SKY_INVALID) most = fmaxf(most, a.r.sigmoid ? fminf(xj[i], 0.0f) : xj[i]);
+    most = group_max_f32<G>(most);
+    float p[KP];
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      p[i] = id[i] == SKY_INVALID ? 0.0f : a.r.sigmoid ? expf(fminf(xj[i], 0.0f) - most) / (1.0f + expf(-fabsf(xj[i]))) : expf(xj[i] - most);
+      all += p[i];
     }
-    if (e < E) dx[e] = (T)v;
+    all = group_sum_f32<G>(all);
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      p[i] = all > 0.0f ? p[i] / all : 0.0f;
+      mean += g[i] * p[i];
+    }
+    mean = group_sum_f32<G>(mean);
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      d[i] = p[i] * (g[i] - mean);
+      if (a.r.sigmoid && id[i] != SKY_INVALID) d[i] *= 1.0f / (1.0f + expf(xj[i]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      d[i] = 0.0f;
+      if (id[i] != SKY_INVALID) d[i] = a.r.sigmoid ? g[i] * (1.0f / (1.0f + expf(-xj[i]))) * (1.0f / (1.0f + expf(xj[i]))) : g[i] * __builtin_amdgcn_exp2f((xj[i] - zmax) * 1.44269504f) / total;
+      mean += d[i];
+    }
+    mean = dense ? group_sum_f32<G>(mean) : 0.0f;
+  }
+  const float weight = dense && total > 0.0f ? -mean / total : 0.0f;
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int e = 0; e < N; e += 4) *(float4*)&part[(i * G + sub) * N + e] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < KP; ++i)
+    if (id[i] != SKY_INVALID) atomicAdd(&part[id[i]], d[i]);  // ids of a row are distinct as they are chosen
+  __builtin_amdgcn_wave_barrier();
+  if (want >= a.rows) return;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const uint32_t c = (i * G + sub) * N;
+    Piece<T> o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o.e[e] = (T)(z[i][e] * weight + part[c + e]);
+    if (c + N <= E) {
+      store_piece(dx + c, o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (c + e < E) dx[c + e] = o.e[e];
+    }
   }
 }
 
@@ -742,6 +810,12 @@ int check_route(const char* who, uint32_t rows, uint32_t experts, const sky_rout
    : experts <= 64 ? launch(kernel<T, 4>)                                                 \
    : experts <= 128 ? launch(kernel<T, 8>)                                                \
                     : launch(kernel<T, 16>))
+#define SKY_ROUTE_PIECES(kernel, T)                     \
+  (lanes == 16 ? (pieces <= 1   ? launch(kernel<T, 16, 1>)  \
+                  : pieces <= 2 ? launch(kernel<T, 16, 2>)  \
+                                : launch(kernel<T, 16, 4>)) \
+               : (pieces <= 2 ? launch(kernel<T, 64, 2>)    \
+                              : launch(kernel<T, 64, 4>)))
 #define SKY_ROUTE_LAUNCH(PER, kernel)       \
   (dtype == SKY_F32 ? PER(kernel, float)    \
    : dtype == SKY_F16 ? PER(kernel, _Float16) \
@@ -828,9 +902,10 @@ extern "C" int sky_route_topk_backward(const void* logits, int dtype, uint32_t r
   a.dlogits = dlogits;
   a.dstride = dlogits_stride;
   const hipStream_t st = (hipStream_t)stream;
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((rows + ROUTE_WAVES - 1) / ROUTE_WAVES), dim3(64 * ROUTE_WAVES), 0, st, a);
-  };
-  SKY_ROUTE_LAUNCH(SKY_ROUTE_PER, route_backward_kernel);
+  // up to 256 experts four rows a wavefront, more one
+  const uint32_t lanes = experts <= QUAD_EXPERTS ? 16 : 64, per_block = 64 / lanes * ROUTE_WAVES;
+  const uint32_t pieces = (uint32_t)((experts * dtype_size(dtype) + 16 * lanes - 1) / (16 * lanes));  // a lane: up to 4
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((rows + per_block - 1) / per_block), dim3(64 * ROUTE_WAVES), 0, st, a); };
+  SKY_ROUTE_LAUNCH(SKY_ROUTE_PIECES, route_backward_kernel);
   return check_launch();
 }
