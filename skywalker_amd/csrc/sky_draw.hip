@@ -540,19 +540,22 @@ struct Reader {
   // reach `least`, and perhaps of others.  Pieces that the maxima name are few, or all are read again and those that are wanted are
   // few; either way an entry of them goes to a thread.  Called by all threads; a barrier is left to the caller.
   template <typename W, typename F>
-  __device__ __forceinline__ void again(Shared& s, uint32_t least, W wanted, F f) const {
+  __device__ __forceinline__ void again(Shared& s, uint32_t least, bool many, W wanted, F f) const {
     const uint32_t raw = least == P::SIGN ? P::SIGN - 1 : least;
-    __syncthreads();
-    if (threadIdx.x == 0) s.hits = 0;
-    __syncthreads();
+    uint32_t hits = HITS + 1, step = TURN;
+    if (!many) {
+      __syncthreads();
+      if (threadIdx.x == 0) s.hits = 0;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i)
-      if (most[i] >= raw) {
-        const uint32_t at = atomicAdd(&s.hits, 1u);
-        if (at < HITS) s.hit[at] = (i * THREADS + threadIdx.x) * N;
-      }
-    __syncthreads();
-    uint32_t hits = s.hits, step = TURN;
+      for (int i = 0; i < PIECES; ++i)
+        if (most[i] >= raw) {
+          const uint32_t at = atomicAdd(&s.hits, 1u);
+          if (at < HITS) s.hit[at] = (i * THREADS + threadIdx.x) * N;
+        }
+      __syncthreads();
+      hits = s.hits;
+    }
     if (hits > HITS) {
       __syncthreads();
       if (threadIdx.x == 0) s.hits = 0;
@@ -586,26 +589,56 @@ struct Reader {
   __device__ __forceinline__ void from(Shared& s, uint32_t least, F f) const {
     const uint32_t raw = least == P::SIGN ? P::SIGN - 1 : least;
     auto some = [&](uint32_t q, uint32_t c) { if (q >= least) f(q, c); };
-    again(s, least, [&](uint4 p) { return piece_max<T>(p) >= raw; }, some);
+    again(s, least, false, [&](uint4 p) { return piece_max<T>(p) >= raw; }, some);
     if (last) some(last, whole + threadIdx.x);
   }
-  // f(column) for the entries of a place
+  // f(column) for the entries of a place; `many`: so many entries are larger that the maxima do not tell where they are
   template <typename F>
-  __device__ __forceinline__ void equal(Shared& s, uint32_t place, F f) const {
+  __device__ __forceinline__ void equal(Shared& s, uint32_t place, bool many, F f) const {
     // what is 0 in a word that holds the place's raw bits; two kinds of bits are the place of 0 and that of the largest number
     const uint32_t other = place == P::SIGN ? P::SIGN - 1 : place == P::LARGEST ? P::LARGEST + 1 : place;
     const uint32_t a = sizeof(T) == 4 ? place : place | place << 16, b = sizeof(T) == 4 ? other : other | other << 16;
     auto some = [&](uint32_t q, uint32_t c) { if (q == place) f(c); };
-    again(s, place, [&](uint4 p) {
+    again(s, place, many, [&](uint4 p) {
       uint32_t m = piece_min<T>(uint4{p.x ^ a, p.y ^ a, p.z ^ a, p.w ^ a});
       if (a != b) m = min(m, piece_min<T>(uint4{p.x ^ b, p.y ^ b, p.z ^ b, p.w ^ b}));
       return m == 0;
     }, some);
     if (last) some(last, whole + threadIdx.x);
   }
-  // f(value, column) for every entry that is there: later readings of the whole row
+  // Entries between two places: f(place, column) for the entries of every piece that holds one, or that holds what is no finite number;
+  // returns how many entries of the other pieces are larger.  All of the row is read.
   template <typename F>
-  __device__ __forceinline__ void all(F f) const {
+  __device__ __forceinline__ uint32_t band(Shared& s, uint32_t lo, uint32_t hi, F f) const {
+    const uint32_t raw = lo == P::SIGN ? P::SIGN - 1 : lo;
+    uint32_t larger = 0;
+    again(s, 0, true, [&](uint4 p) {
+      if (piece_max<T>(p) > P::LARGEST) return true;
+      uint32_t in = 0, over = 0;
+      auto one = [&](uint32_t q) {
+        in |= q - raw <= hi - raw;
+        over += q > hi;
+      };
+      const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          one(w[i]);
+        } else {
+          one(w[i] & 0xFFFFu);
+          one(w[i] >> 16);
+        }
+      }
+      larger += in ? 0 : over;
+      return in != 0;
+    }, f);
+    if (last) f(last, whole + threadIdx.x);
+    return larger;
+  }
+  // f(value) for every entry from `low` on: later readings of the whole row
+  template <typename F>
+  __device__ __forceinline__ void values(float low, F f) const {
+    const uint32_t least = place_of((T)low), raw = least == P::SIGN ? P::SIGN - 1 : least;
 #pragma unroll 1
     for (uint32_t c = threadIdx.x * N; c < whole; c += 8 * STEP) {
       uint4 w[8];
@@ -616,34 +649,30 @@ struct Reader {
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t at = c + i * STEP;
         if (at < whole) {
-          if constexpr (sizeof(T) == 4) {
-            // NaN and -inf pass no test of a value, +inf is the largest number
-            auto one = [&](uint32_t bits, uint32_t col) {
-              const float z = __uint_as_float(bits);
-              f((z > 3.402823466e38f ? 3.402823466e38f : z) + 0.0f, col);  // -0 is 0
-            };
-            one(w[i].x, at);
-            one(w[i].y, at + 1);
-            one(w[i].z, at + 2);
-            one(w[i].w, at + 3);
+          const uint4 p = raw_places<T>(w[i]);
+          if (sizeof(T) == 4 && piece_max<T>(p) <= P::LARGEST && piece_min<T>(p) >= raw && least) {
+            f(__uint_as_float(w[i].x));
+            f(__uint_as_float(w[i].y));
+            f(__uint_as_float(w[i].z));
+            f(__uint_as_float(w[i].w));
           } else {
-            each<T>(w[i], at, [&](uint32_t q, uint32_t col) { if (q) f(P::value(q), col); });
+            each<T>(w[i], at, [&](uint32_t q, uint32_t) { if (q && P::value(q) >= low) f(P::value(q)); });
           }
         }
       }
     }
-    if (last) f(P::value(last), whole + threadIdx.x);
+    if (last && P::value(last) >= low) f(P::value(last));
   }
 };
 
 // The column of entry `tie` among those of value z, by column: as few of them as the list holds are listed, more are counted off.
 template <typename T>
-__device__ __forceinline__ uint32_t column_of_tie(const Reader<T>& in, Shared& s, uint32_t q, uint32_t tie, uint32_t ties) {
+__device__ __forceinline__ uint32_t column_of_tie(const Reader<T>& in, Shared& s, uint32_t q, uint32_t tie, uint32_t ties, uint64_t larger) {
   __syncthreads();
   if (threadIdx.x == 0) s.found = SKY_INVALID;
   if (ties <= CAP) {
     if (threadIdx.x == 0) s.place = 0;
-    in.equal(s, q, [&](uint32_t c) { s.room[atomicAdd(&s.place, 1u)] = c; });
+    in.equal(s, q, larger > 4 * HITS, [&](uint32_t c) { s.room[atomicAdd(&s.place, 1u)] = c; });
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < ties; i += THREADS) {
       uint32_t below = 0;
@@ -842,7 +871,7 @@ __device__ __forceinline__ bool draw_by_value(const Reader<T>& in, Shared& s, co
     }
   }
   const ValuePlace p = locate_value<false, T>(s, row, Row::drawn(u, mass), count_before, mass_before);
-  *result = Result{column_of_tie(in, s, p.q, p.tie, count_of(c, p.q)), count, row.log_share(p.z, mass)};
+  *result = Result{column_of_tie(in, s, p.q, p.tie, count_of(c, p.q), p.count_before), count, row.log_share(p.z, mass)};
   return true;
 }
 
@@ -856,10 +885,14 @@ struct Bins {
     narrow = scale > 1e-30 && scale < 1e30 ? (float)scale : 0.0f;
   }
   __device__ __forceinline__ bool has(float z) const { return z <= top && z >= low; }
-  // no value of bins 0 .. b is smaller
-  __device__ __forceinline__ float edge(uint32_t b) const {
+  // no value of bins 0 .. b is smaller than the lower edge, none of bins b and on is larger than the upper one
+  __device__ __forceinline__ float lower_edge(uint32_t b) const {
     const double z = scale > 0.0 ? hi - ((double)b + 1.0) / scale : (double)low;
-    return fmaxf((float)(z - 1e-5 * fabs(z) - 1e-5 * ((double)top - z)), low);
+    return fmaxf((float)(z - 1e-6 * fabs(z) - 1e-5 * ((double)top - z)), low);
+  }
+  __device__ __forceinline__ float upper_edge(uint32_t b) const {
+    const double z = scale > 0.0 ? hi - (double)b / scale : (double)top;
+    return fminf((float)(z + 1e-6 * fabs(z) + 1e-5 * ((double)top - z)), top);
   }
   __device__ __forceinline__ uint32_t of(float z) const {
     return min(narrow != 0.0f ? (uint32_t)((top - z) * narrow) : (uint32_t)((hi - (double)z) * scale), BINS - 1);
@@ -884,11 +917,8 @@ __device__ __forceinline__ Filled fill_bins(const Reader<T>& in, Shared& s, cons
   __syncthreads();
   s.bin[2 * threadIdx.x] = s.bin[2 * threadIdx.x + 1] = 0;
   __syncthreads();
-  in.all([&](float z, uint32_t) {
-    if (bins.has(z)) {
-      const uint64_t v = value(z);
-      if (v) atomicAdd((unsigned long long*)&s.bin[bins.of(z)], (unsigned long long)v);
-    }
+  in.values(bins.low, [&](float z) {
+    if (z <= bins.top) atomicAdd((unsigned long long*)&s.bin[bins.of(z)], (unsigned long long)value(z));
   });
   __syncthreads();
   if (excess && bins.has(low) && threadIdx.x == 0) s.bin[bins.of(low)] -= (uint64_t)excess * value(low);
@@ -902,6 +932,7 @@ __device__ __forceinline__ Filled fill_bins(const Reader<T>& in, Shared& s, cons
 // The entry that holds unit `unit`, from the bins of the whole interval.  Every thread calls it and has the answer.
 template <bool RANK, typename T>
 __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Row& row, Bins bins, Filled f, float low, uint32_t excess, uint64_t unit) {
+  using P = Places<T>;
   auto value = [&](float z) -> uint64_t { return RANK ? 1ull : row.units(z); };
   Place p;
   uint64_t before = 0;
@@ -924,13 +955,15 @@ __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Ro
     // the bin's entries: how many, between which values, and the list of them if it holds them; and how many entries are larger
     uint32_t kmin = 0xFFFFFFFFu, kmax = 0;
     uint64_t larger = 0;
-    in.from(s, place_of((T)bins.edge(b)), [&](uint32_t q, uint32_t c) {
-      const float z = Places<T>::value(q);
+    uint32_t in_pieces = 0;
+    larger = in.band(s, max(place_of((T)bins.lower_edge(b)), P::LOWEST), place_of((T)bins.upper_edge(b)), [&](uint32_t q, uint32_t c) {
+      if (!q) return;
+      const float z = P::value(q);
       if (z > bins.top) {
-        ++larger;
+        ++in_pieces;
       } else if (z >= bins.low) {
         const uint32_t mine = bins.of(z);
-        larger += mine < b;
+        in_pieces += mine < b;
         if (mine == b) {
           const uint32_t key = score_key(z), at = atomicAdd(&s.l.n, 1u);
           kmin = min(kmin, key);
@@ -939,6 +972,7 @@ __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Ro
         }
       }
     });
+    larger += in_pieces;
     kmin = wave_min_u32(kmin);
     kmax = wave_max_u32(kmax);
     if ((threadIdx.x & 63) == 0 && kmax) {
@@ -1019,11 +1053,9 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, c
     const uint32_t least = min(last_failing<T>(most, [&](float z) { return row.weight(z) >= (double)o.min_p; }) + 1, most);
     const float z_least = Places<T>::value(max(least, Places<T>::LOWEST));
     uint64_t weighs = 0, many = 0, all, all_many;
-    in.all([&](float z, uint32_t) {
-      if (z >= z_least) {
-        weighs += row.units(z);
-        ++many;
-      }
+    in.values(z_least, [&](float z) {
+      weighs += row.units(z);
+      ++many;
     });
     block_scan<THREADS>(weighs, s.wave, &all);
     block_scan<THREADS>(many, s.wave, &all_many);
@@ -1035,7 +1067,7 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, c
   const Place p = locate<false>(in, s, row, bins, f, low, excess, Row::drawn(u, mass));
   Result r{p.column, count, row.log_share(p.z, mass)};
   if (r.token == SKY_INVALID) {
-    r.token = column_of_tie(in, s, place_of((T)p.z), p.tie, p.ties);
+    r.token = column_of_tie(in, s, place_of((T)p.z), p.tie, p.ties, p.larger);
   }
   return r;
 }
@@ -1119,7 +1151,7 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared&
   if (!there) return nothing_to_draw();
   if (greedy) {
     if (threadIdx.x == 0) s.place = SKY_INVALID;
-    in.equal(s, most, [&](uint32_t c) { atomicMin(&s.place, c); });
+    in.equal(s, most, false, [&](uint32_t c) { atomicMin(&s.place, c); });
     __syncthreads();
     return Result{s.place, 1, 0.0};
   }
