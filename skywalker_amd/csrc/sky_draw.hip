@@ -536,6 +536,27 @@ struct Reader {
     for (int i = 0; i < PIECES; ++i) m = max(m, most[i]);
     return max(m == P::SIGN - 1 ? P::SIGN : m, last);  // -0
   }
+  // f(a piece's bits, column) for all pieces: AHEAD of them are under way while as many are worked on
+  template <typename F>
+  __device__ __forceinline__ void stream(F f) const {
+    uint4 w[2][AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) w[0][i] = load(i * STEP + threadIdx.x * N);
+#pragma unroll 1
+    for (uint32_t base = 0; base < whole; base += 2 * AHEAD * STEP)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) w[1 - h][i] = load(base + ((h + 1) * AHEAD + i) * STEP + threadIdx.x * N);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          const uint32_t c = base + (h * AHEAD + i) * STEP + threadIdx.x * N;
+          if (c < whole) f(w[h][i], c);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
   // f(place, column) for every entry of the pieces that `wanted` (of a piece's raw places) says yes to, of those whose largest place may
   // reach `least`, and perhaps of others.  Pieces that the maxima name are few, or all are read again and those that are wanted are
   // few; either way an entry of them goes to a thread.  Called by all threads; a barrier is left to the caller.
@@ -560,23 +581,15 @@ struct Reader {
       __syncthreads();
       if (threadIdx.x == 0) s.hits = 0;
       __syncthreads();
-#pragma unroll 1
-      for (uint32_t c = threadIdx.x * N; c < whole; c += 8 * STEP) {
-        uint4 w[8];
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) w[i] = load(c + i * STEP);
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-          const uint32_t at_column = c + i * STEP;
-          if (at_column < whole && wanted(raw_places<T>(w[i]))) {
-            const uint32_t at = atomicAdd(&s.hits, 1u);
-            if (at < HITS)
-              s.hit[at] = at_column;
-            else
-              each<T>(w[i], at_column, f);  // not few
-          }
+      stream([&](uint4 w, uint32_t c) {
+        if (wanted(raw_places<T>(w))) {
+          const uint32_t at = atomicAdd(&s.hits, 1u);
+          if (at < HITS)
+            s.hit[at] = c;
+          else
+            each<T>(w, c, f);  // not few
         }
-      }
+      });
       __syncthreads();
       hits = min(s.hits, HITS);
       step = whole;
@@ -639,28 +652,17 @@ struct Reader {
   template <typename F>
   __device__ __forceinline__ void values(float low, F f) const {
     const uint32_t least = place_of((T)low), raw = least == P::SIGN ? P::SIGN - 1 : least;
-#pragma unroll 1
-    for (uint32_t c = threadIdx.x * N; c < whole; c += 8 * STEP) {
-      uint4 w[8];
-#pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) w[i] = load(c + i * STEP);
-#pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) {
-        __builtin_amdgcn_sched_barrier(0);
-        const uint32_t at = c + i * STEP;
-        if (at < whole) {
-          const uint4 p = raw_places<T>(w[i]);
-          if (sizeof(T) == 4 && piece_max<T>(p) <= P::LARGEST && piece_min<T>(p) >= raw && least) {
-            f(__uint_as_float(w[i].x));
-            f(__uint_as_float(w[i].y));
-            f(__uint_as_float(w[i].z));
-            f(__uint_as_float(w[i].w));
-          } else {
-            each<T>(w[i], at, [&](uint32_t q, uint32_t) { if (q && P::value(q) >= low) f(P::value(q)); });
-          }
-        }
+    stream([&](uint4 w, uint32_t c) {
+      const uint4 p = raw_places<T>(w);
+      if (sizeof(T) == 4 && piece_max<T>(p) <= P::LARGEST && piece_min<T>(p) >= raw && least) {
+        f(__uint_as_float(w.x));
+        f(__uint_as_float(w.y));
+        f(__uint_as_float(w.z));
+        f(__uint_as_float(w.w));
+      } else {
+        each<T>(w, c, [&](uint32_t q, uint32_t) { if (q && P::value(q) >= low) f(P::value(q)); });
       }
-    }
+    });
     if (last && P::value(last) >= low) f(P::value(last));
   }
 };
