@@ -4,12 +4,11 @@
 // everything is one question, asked up to three times: which entry of the order holds rank k, or the unit of mass t?  A row is read
 // once to answer it, and in places a second time; it is never sorted.  What is done depends on how many entries can matter:
 //
-//   list    at most CAP entries can stay: they are listed in LDS and sorted.  Short rows, rows of which a grammar leaves a few
-//           (draw_short_kernel, several rows to a CU), and, in rows of any length, top-k of up to SMALL_K (the k-th largest of the
-//           threads' largest entries is no larger than the k-th largest entry) and min-p without top-p.
+//   list    at most CAP entries can stay: they are listed in LDS and sorted.  Rows of which a grammar leaves a few, top-k of up to
+//           SMALL_K (the k-th largest of the threads' largest entries is no larger than the k-th largest entry) and min-p without top-p.
 //   values  16-bit logits have at most 65,536 values: they are counted by value, in 16-bit counters that take 128 KB of
 //           LDS, and the rest (weights, prefixes, borders) is a matter of the values that occur, a few thousand.
-//   bins    fp32, and rows in which a counter runs over: weights are summed in BINS bins of equal width between the largest
+//   bins    the others (fp32, shorter rows, rows in which a counter runs over): weights are summed in BINS bins of equal width between the largest
 //           value and the smallest that weighs anything; the bin that holds the answer is listed and sorted, and
 //           when it does not fit the list it becomes the next interval.  That then lies between the smallest and largest value met in it, so
 //           that two different values never stay together, and a bin of one value is a matter of counting.
@@ -23,14 +22,15 @@ namespace sky {
 namespace {
 
 constexpr int THREADS = 1024;        // of a workgroup that has a CU to itself
-constexpr int SHORT_THREADS = 256;   // of a workgroup for a short row
-constexpr uint32_t BINS = 2048;      // two per thread
-constexpr uint32_t CAP = 2048;       // entries of a list
+constexpr int SHORT_THREADS = 256;   // of a workgroup for a shorter row
+constexpr uint32_t BINS = 2048;
+template <int BT>
+constexpr uint32_t CAP = 2 * BT;     // entries of a list: two per thread of the workgroup
 constexpr double NO_MASS = 40.0;     // weights below e^-40 are 0 in units of 2^-S, S <= 50
-constexpr uint32_t SMALL_K = 512;    // of the 1024 threads' largest entries: some 710 entries are as large as the 512th of them
+template <int BT>
+constexpr uint32_t SMALL_K = BT / 2;  // of 1024 threads' largest entries: some 710 entries are as large as the 512th of them
 constexpr uint32_t VALUES = 65536, CHUNK = 256, CHUNKS = VALUES / CHUNK;  // of 16-bit logits; a wavefront takes a chunk, four values a lane
 constexpr int PIECES = 16, AHEAD = 4;  // pieces of 16 bytes that a thread tells apart, and of a load that runs while as many are worked on
-constexpr uint32_t HITS = THREADS;   // pieces that are read a second time one by one; more: the whole row is
 constexpr uint32_t MAX_COLUMNS = 1u << 26;  // a thread counts its elements in 16 bits
 constexpr uint32_t NOT_DRAWN = 0xFFFFFFFEu;  // token of a row that draw_short_kernel leaves to draw_kernel
 
@@ -64,6 +64,10 @@ struct Settings {
     if (!(min_p > 0.0f)) min_p = 0.0f;
   }
   __device__ __forceinline__ bool greedy() const { return !(temperature > 0.0f); }
+  // few entries can stay: top-k of up to `small_k`, and where `by_min_p` min-p without top-p
+  __device__ __forceinline__ bool few(uint32_t small_k, bool by_min_p) const {
+    return greedy() || (top_k && top_k <= small_k) || (by_min_p && min_p > 0.0f && !(top_p < 1.0f));
+  }
 };
 __device__ __forceinline__ double uniform_of(const DrawArgs& a, uint32_t r) {
   if (a.uniforms) return fmax(a.uniforms[r], 0.0);
@@ -250,7 +254,7 @@ constexpr uint64_t LIST_END = ~0ull;
 
 template <int BT>
 struct ListShared {
-  uint64_t list[CAP];
+  uint64_t list[CAP<BT>];
   uint64_t wave[BT / 64];
   uint64_t before;
   uint32_t n, found;
@@ -342,7 +346,7 @@ __device__ __forceinline__ Result draw_wave(uint64_t* list, uint32_t n, const Se
 // The same for m > 64 entries of s.list (or fewer), by the workgroup.
 template <int BT>
 __device__ __forceinline__ Result draw_listed(ListShared<BT>& s, uint32_t m, const Settings& o, double u) {
-  constexpr uint32_t PER = CAP / BT;
+  constexpr uint32_t PER = CAP<BT> / BT;
   sort_list<BT>(s.list, m);
   const Row row(o.temperature, listed_score(s.list[0]), 50);  // at most 2^11 weights
   const uint32_t k = o.top_k && o.top_k < m ? o.top_k : m, i0 = PER * threadIdx.x;
@@ -404,89 +408,72 @@ __device__ __forceinline__ Result first_listed(ListShared<BT>& s, uint32_t n) {
   return Result{(uint32_t)best, 1, 0.0};
 }
 
-// ---------------------------------------------------------------- short rows, and rows with little in them
-// A workgroup of four wavefronts, so that several rows are on a CU and one's loads run beside another's sort.  SPARSE: rows of more
-// than CAP entries, most of which are not there; one that has many after all, which its first columns tell, is left to draw_kernel.
-template <typename T, bool SPARSE>
-__global__ __launch_bounds__(SHORT_THREADS) void draw_short_kernel(DrawArgs a) {
-  constexpr uint32_t N = Piece<T>::N, STEP = SHORT_THREADS * N, LOADS = 8;
-  using P = Places<T>;
-  __shared__ ListShared<SHORT_THREADS> s;
-  const uint32_t r = blockIdx.x, tid = threadIdx.x, columns = a.columns, whole = columns / N * N;
-  const T* const x = (const T*)a.logits + r * a.stride;
-  if (tid == 0) s.n = 0;
-  __syncthreads();
-  auto put = [&](uint32_t q, uint32_t c) {
-    if (q) {
-      const uint32_t at = atomicAdd(&s.n, 1u);
-      if (at < CAP) s.list[at] = listed(P::value(q), c);
-    }
+// A place that at least k of the `counts` values v[i] of the wavefront's lanes reach, and few more (MAX of them are looked at: `counts`
+// of a lane; the others are left alone).  `most`: the largest.
+template <int MAX>
+__device__ __forceinline__ uint32_t place_of_rank(const uint32_t (&v)[MAX], int counts, uint32_t k, uint32_t most) {
+  auto reach = [&](uint32_t place) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < MAX; ++i)
+      if (i < counts) n += (uint32_t)__builtin_popcountll(__ballot(v[i] >= place));
+    return n;
   };
-  auto piece = [&](uint4 w, uint32_t c) {
-    if (piece_max<T>(raw_places<T>(w)) >= P::LOWEST) each<T>(w, c, put);
-  };
-  uint32_t c0 = 0;
-  if (SPARSE) {
-    piece(load_words(x + tid * N), tid * N);
-    c0 = STEP;
-    __syncthreads();
-    const uint32_t seen = s.n;
-    __syncthreads();
-    if ((uint64_t)seen * columns > (uint64_t)2 * CAP * STEP) {
-      if (tid == 0) a.tokens[r * a.tokens_stride] = NOT_DRAWN;
-      return;
+  uint32_t lo = v[0], hi = most;  // k or more reach lo, fewer reach more than hi
+#pragma unroll
+  for (int i = 1; i < MAX; ++i)
+    if (i < counts) lo = min(lo, v[i]);
+  lo = wave_min_u32(lo);  // all of them reach it
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2, n = reach(mid);
+    if (n >= k) {
+      lo = mid;
+      if (n <= k + 16) break;
+    } else {
+      hi = mid - 1;
     }
   }
-  for (; c0 + LOADS * STEP <= whole; c0 += LOADS * STEP) {
-    uint4 w[LOADS];
-#pragma unroll
-    for (uint32_t i = 0; i < LOADS; ++i) w[i] = load_words(x + c0 + i * STEP + tid * N);
-#pragma unroll
-    for (uint32_t i = 0; i < LOADS; ++i) piece(w[i], c0 + i * STEP + tid * N);
-  }
-  for (uint32_t c = c0 + tid * N; c < whole; c += STEP) piece(load_words(x + c), c);
-  if (whole + tid < columns) put(place_of(x[whole + tid]), whole + tid);
-  __syncthreads();
-  const uint32_t n = s.n;
-  if (SPARSE && n > CAP) {
-    if (tid == 0) a.tokens[r * a.tokens_stride] = NOT_DRAWN;
-    return;
-  }
-  Result d = nothing_to_draw();
-  if (n) {
-    const Settings o(a, r);
-    d = o.greedy() ? first_listed(s, n) : draw_list(s, n, o, uniform_of(a, r));
-  }
-  if (tid == 0) store_result(a, r, d);
+  return lo;
 }
 
-// ---------------------------------------------------------------- a row a CU
+// ---------------------------------------------------------------- a row a workgroup
 struct Counters {
   uint32_t value[VALUES / 2];  // places below 32,768 in the low halves, the others in the high ones
   uint32_t chunk_count[CHUNKS];
   uint64_t chunk_mass[CHUNKS];
 };
+template <int BT>
+struct BinsAndList {
+  ListShared<BT> l;
+  uint64_t bin[BINS];
+};
+template <int BT>
+union Large {
+  BinsAndList<BT> some;
+};
+template <>
+union Large<THREADS> {
+  BinsAndList<THREADS> some;
+  Counters counters;  // of 16-bit logits
+};
+// LDS of a workgroup of BT threads: one of 1024 has a CU to itself, of 256 four are on one.
+template <int BT>
 struct Shared {
-  union {
-    struct {
-      ListShared<THREADS> l;
-      uint64_t bin[BINS];
-    };
-    Counters counters;
-  };
-  uint64_t wave[THREADS / 64];
+  Large<BT> large;
+  uint64_t wave[BT / 64];
   uint64_t count_before, mass_before;
-  uint32_t most[THREADS], hit[HITS], room[CAP];
-  uint32_t wave_most[THREADS / 64], wave_least[THREADS / 64], wave_there[THREADS / 64], wave_above[THREADS / 64];
+  uint32_t most[BT], hit[BT], room[CAP<BT>];
+  uint32_t wave_most[BT / 64], wave_least[BT / 64], wave_there[BT / 64], wave_above[BT / 64];
   uint32_t hits, place, chunk, found, lo, hi;
 };
-static_assert(sizeof(Shared) <= 160 * 1024, "LDS of a CU");
+static_assert(sizeof(Shared<THREADS>) <= 160 * 1024 && sizeof(Shared<SHORT_THREADS>) <= 40 * 1024, "LDS of a CU");
 
-// A row as the workgroup's threads read it: PIECES each in turns of THREADS * PIECES, and an entry each of those that do
+// A row as the workgroup's threads read it: PIECES each in turns of BT * PIECES, and an entry each of those that do
 // not fill a piece.  Kept of it: the largest raw place of each of a thread's pieces (over all turns).
-template <typename T>
+template <typename T, int BT>
 struct Reader {
-  static constexpr uint32_t N = Piece<T>::N, STEP = THREADS * N, TURN = STEP * PIECES;
+  static constexpr uint32_t N = Piece<T>::N, STEP = BT * N, TURN = STEP * PIECES;
+  static constexpr uint32_t HITS = BT;  // pieces that are read a second time an entry a thread
   using P = Places<T>;
   const T* x;
   uint32_t columns, whole;
@@ -503,8 +490,9 @@ struct Reader {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) most[i] = 0;
     uint4 w[2][AHEAD];  // those that are worked on, and those that are under way
+    if (whole)
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) w[0][i] = load(i * STEP + threadIdx.x * N);
+      for (int i = 0; i < AHEAD; ++i) w[0][i] = load(i * STEP + threadIdx.x * N);
 #pragma unroll 1
     for (uint32_t turn = 0; turn < whole; turn += TURN) {
 #pragma unroll
@@ -540,6 +528,7 @@ struct Reader {
   template <typename F>
   __device__ __forceinline__ void stream(F f) const {
     uint4 w[2][AHEAD];
+    if (!whole) return;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) w[0][i] = load(i * STEP + threadIdx.x * N);
 #pragma unroll 1
@@ -561,7 +550,7 @@ struct Reader {
   // reach `least`, and perhaps of others.  Pieces that the maxima name are few, or all are read again and those that are wanted are
   // few; either way an entry of them goes to a thread.  Called by all threads; a barrier is left to the caller.
   template <typename W, typename F>
-  __device__ __forceinline__ void again(Shared& s, uint32_t least, bool many, W wanted, F f) const {
+  __device__ __forceinline__ void again(Shared<BT>& s, uint32_t least, bool many, W wanted, F f) const {
     const uint32_t raw = least == P::SIGN ? P::SIGN - 1 : least;
     uint32_t hits = HITS + 1, step = TURN;
     if (!many) {
@@ -572,7 +561,7 @@ struct Reader {
       for (int i = 0; i < PIECES; ++i)
         if (most[i] >= raw) {
           const uint32_t at = atomicAdd(&s.hits, 1u);
-          if (at < HITS) s.hit[at] = (i * THREADS + threadIdx.x) * N;
+          if (at < HITS) s.hit[at] = (i * BT + threadIdx.x) * N;
         }
       __syncthreads();
       hits = s.hits;
@@ -594,12 +583,12 @@ struct Reader {
       hits = min(s.hits, HITS);
       step = whole;
     }
-    for (uint32_t i = threadIdx.x; i < hits * N; i += THREADS)
+    for (uint32_t i = threadIdx.x; i < hits * N; i += BT)
       for (uint32_t c = s.hit[i / N] + i % N; c < whole; c += step) f(place_of(x[c]), c);
   }
   // f(place, column) for the entries from `least` on
   template <typename F>
-  __device__ __forceinline__ void from(Shared& s, uint32_t least, F f) const {
+  __device__ __forceinline__ void from(Shared<BT>& s, uint32_t least, F f) const {
     const uint32_t raw = least == P::SIGN ? P::SIGN - 1 : least;
     auto some = [&](uint32_t q, uint32_t c) { if (q >= least) f(q, c); };
     again(s, least, false, [&](uint4 p) { return piece_max<T>(p) >= raw; }, some);
@@ -607,7 +596,7 @@ struct Reader {
   }
   // f(column) for the entries of a place; `many`: so many entries are larger that the maxima do not tell where they are
   template <typename F>
-  __device__ __forceinline__ void equal(Shared& s, uint32_t place, bool many, F f) const {
+  __device__ __forceinline__ void equal(Shared<BT>& s, uint32_t place, bool many, F f) const {
     // what is 0 in a word that holds the place's raw bits; two kinds of bits are the place of 0 and that of the largest number
     const uint32_t other = place == P::SIGN ? P::SIGN - 1 : place == P::LARGEST ? P::LARGEST + 1 : place;
     const uint32_t a = sizeof(T) == 4 ? place : place | place << 16, b = sizeof(T) == 4 ? other : other | other << 16;
@@ -622,7 +611,7 @@ struct Reader {
   // Entries between two places: f(place, column) for the entries of every piece that holds one, or that holds what is no finite number;
   // returns how many entries of the other pieces are larger.  All of the row is read.
   template <typename F>
-  __device__ __forceinline__ uint32_t band(Shared& s, uint32_t lo, uint32_t hi, F f) const {
+  __device__ __forceinline__ uint32_t band(Shared<BT>& s, uint32_t lo, uint32_t hi, F f) const {
     const uint32_t raw = lo == P::SIGN ? P::SIGN - 1 : lo;
     uint32_t larger = 0;
     again(s, 0, true, [&](uint4 p) {
@@ -654,11 +643,21 @@ struct Reader {
     const uint32_t least = place_of((T)low), raw = least == P::SIGN ? P::SIGN - 1 : least;
     stream([&](uint4 w, uint32_t c) {
       const uint4 p = raw_places<T>(w);
-      if (sizeof(T) == 4 && piece_max<T>(p) <= P::LARGEST && piece_min<T>(p) >= raw && least) {
-        f(__uint_as_float(w.x));
-        f(__uint_as_float(w.y));
-        f(__uint_as_float(w.z));
-        f(__uint_as_float(w.w));
+      // (16-bit rows of a workgroup of 1024 come here only if their counters run over: they go without)
+      if ((sizeof(T) == 4 || BT != THREADS) && piece_max<T>(p) <= P::LARGEST && piece_min<T>(p) >= raw && least) {
+        if constexpr (sizeof(T) == 4) {
+          f(__uint_as_float(w.x));
+          f(__uint_as_float(w.y));
+          f(__uint_as_float(w.z));
+          f(__uint_as_float(w.w));
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            f((float)__builtin_bit_cast(T, (uint16_t)w.x));
+            f((float)__builtin_bit_cast(T, (uint16_t)(w.x >> 16)));
+            w = uint4{w.y, w.z, w.w, 0};
+          }
+        }
       } else {
         each<T>(w, c, [&](uint32_t q, uint32_t) { if (q && P::value(q) >= low) f(P::value(q)); });
       }
@@ -668,15 +667,15 @@ struct Reader {
 };
 
 // The column of entry `tie` among those of value z, by column: as few of them as the list holds are listed, more are counted off.
-template <typename T>
-__device__ __forceinline__ uint32_t column_of_tie(const Reader<T>& in, Shared& s, uint32_t q, uint32_t tie, uint32_t ties, uint64_t larger) {
+template <typename T, int BT>
+__device__ __forceinline__ uint32_t column_of_tie(const Reader<T, BT>& in, Shared<BT>& s, uint32_t q, uint32_t tie, uint32_t ties, uint64_t larger) {
   __syncthreads();
   if (threadIdx.x == 0) s.found = SKY_INVALID;
-  if (ties <= CAP) {
+  if (ties <= CAP<BT>) {
     if (threadIdx.x == 0) s.place = 0;
-    in.equal(s, q, larger > 4 * HITS, [&](uint32_t c) { s.room[atomicAdd(&s.place, 1u)] = c; });
+    in.equal(s, q, larger > 4 * BT, [&](uint32_t c) { s.room[atomicAdd(&s.place, 1u)] = c; });
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < ties; i += THREADS) {
+    for (uint32_t i = threadIdx.x; i < ties; i += BT) {
       uint32_t below = 0;
       const uint32_t c = s.room[i];
       for (uint32_t j = 0; j < ties; ++j) below += s.room[j] < c;
@@ -684,11 +683,11 @@ __device__ __forceinline__ uint32_t column_of_tie(const Reader<T>& in, Shared& s
     }
   } else {
     uint64_t seen = 0;
-    for (uint32_t base = 0; base < in.columns && seen <= tie; base += THREADS) {
+    for (uint32_t base = 0; base < in.columns && seen <= tie; base += BT) {
       const uint32_t c = base + threadIdx.x;
       const uint64_t here = c < in.columns && place_of(in.x[c]) == q;
       uint64_t total;
-      const uint64_t before = seen + block_scan<THREADS>(here, s.wave, &total);
+      const uint64_t before = seen + block_scan<BT>(here, s.wave, &total);
       if (here && before == tie) s.found = c;
       seen += total;
     }
@@ -736,12 +735,12 @@ struct ValuePlace {
   __device__ __forceinline__ uint64_t mass_with() const { return mass_before + (uint64_t)(tie + 1) * each; }
 };
 template <bool RANK, typename T>
-__device__ __forceinline__ ValuePlace locate_value(Shared& s, const Row& row, uint64_t unit, uint64_t count_before, uint64_t mass_before) {
+__device__ __forceinline__ ValuePlace locate_value(Shared<THREADS>& s, const Row& row, uint64_t unit, uint64_t count_before, uint64_t mass_before) {
   __syncthreads();
   if (threadIdx.x < CHUNKS) {
     const uint32_t mine = CHUNKS - 1 - threadIdx.x;
     const uint64_t before = RANK ? count_before : mass_before;
-    const uint64_t here = RANK ? (uint64_t)s.counters.chunk_count[mine] : s.counters.chunk_mass[mine];
+    const uint64_t here = RANK ? (uint64_t)s.large.counters.chunk_count[mine] : s.large.counters.chunk_mass[mine];
     if (before <= unit && unit < before + here) {
       s.chunk = mine;
       s.count_before = count_before;
@@ -750,7 +749,7 @@ __device__ __forceinline__ ValuePlace locate_value(Shared& s, const Row& row, ui
   }
   __syncthreads();
   Values v;
-  values_of(s.counters, s.chunk, &v);
+  values_of(s.large.counters, s.chunk, &v);
   weigh<T>(row, &v);
   uint64_t counts = s.count_before + group_scan_u32<64>(v.counts()) - v.counts(), masses = s.mass_before + group_scan_u64<64>(v.masses()) - v.masses();
   ValuePlace p{0, 0, 0.0f, 0, 0, 0};
@@ -799,10 +798,10 @@ __device__ __forceinline__ void count_word(Counters& c, uint32_t w) {
 // A row that has been counted, all but entries of the lowest value, which masks are made of: `above` of `there`.  false: a counter
 // has run over, or the lowest value weighs something.
 template <typename T>
-__device__ __forceinline__ bool draw_by_value(const Reader<T>& in, Shared& s, const Row& row, const Settings& o, double u, uint32_t most, uint32_t there,
+__device__ __forceinline__ bool draw_by_value(const Reader<T, THREADS>& in, Shared<THREADS>& s, const Row& row, const Settings& o, double u, uint32_t most, uint32_t there,
                                               uint32_t above, Result* result) {
   using P = Places<T>;
-  Counters& c = s.counters;
+  Counters& c = s.large.counters;
   if (there != above && row.units(P::value(P::LOWEST))) return false;
   if (threadIdx.x == 0) {  // what was counted as -0 is 0
     const uint32_t n = c.value[P::SIGN - 1] & 0xFFFFu;
@@ -907,33 +906,36 @@ struct Place {
   uint32_t tie, ties, column;
   uint64_t before, larger;  // `larger`: entries before the value
 };
-// What a thread knows of the bins it owns, 2 t and 2 t + 1.
+// What a thread knows of the bins it owns, BINS / BT of them.
+template <int BT>
 struct Filled {
-  uint64_t before, b0, b1, total;
+  static constexpr uint32_t PER = BINS / BT;
+  uint64_t before, bin[PER], all, total;
 };
 
 // The values, RANK: entries; else units of mass, of the entries of [low, zmax], less `excess` entries of the value `low`, in bins.
-template <bool RANK, typename T>
-__device__ __forceinline__ Filled fill_bins(const Reader<T>& in, Shared& s, const Row& row, const Bins& bins, float low, uint32_t excess) {
+template <bool RANK, typename T, int BT>
+__device__ __forceinline__ Filled<BT> fill_bins(const Reader<T, BT>& in, Shared<BT>& s, const Row& row, const Bins& bins, float low, uint32_t excess) {
   auto value = [&](float z) -> uint64_t { return RANK ? 1ull : row.units(z); };
   __syncthreads();
-  s.bin[2 * threadIdx.x] = s.bin[2 * threadIdx.x + 1] = 0;
+  for (uint32_t i = threadIdx.x; i < BINS; i += BT) s.large.some.bin[i] = 0;
   __syncthreads();
   in.values(bins.low, [&](float z) {
-    if (z <= bins.top) atomicAdd((unsigned long long*)&s.bin[bins.of(z)], (unsigned long long)value(z));
+    if (z <= bins.top) atomicAdd((unsigned long long*)&s.large.some.bin[bins.of(z)], (unsigned long long)value(z));
   });
   __syncthreads();
-  if (excess && bins.has(low) && threadIdx.x == 0) s.bin[bins.of(low)] -= (uint64_t)excess * value(low);
+  if (excess && bins.has(low) && threadIdx.x == 0) s.large.some.bin[bins.of(low)] -= (uint64_t)excess * value(low);
   __syncthreads();
-  Filled f;
-  f.b0 = s.bin[2 * threadIdx.x];
-  f.b1 = s.bin[2 * threadIdx.x + 1];
-  f.before = block_scan<THREADS>(f.b0 + f.b1, s.wave, &f.total);
+  Filled<BT> f;
+  f.all = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < f.PER; ++i) f.all += f.bin[i] = s.large.some.bin[f.PER * threadIdx.x + i];
+  f.before = block_scan<BT>(f.all, s.wave, &f.total);
   return f;
 }
 // The entry that holds unit `unit`, from the bins of the whole interval.  Every thread calls it and has the answer.
-template <bool RANK, typename T>
-__device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Row& row, Bins bins, Filled f, float low, uint32_t excess, uint64_t unit) {
+template <bool RANK, typename T, int BT>
+__device__ __forceinline__ Place locate(const Reader<T, BT>& in, Shared<BT>& s, const Row& row, Bins bins, Filled<BT> f, float low, uint32_t excess, uint64_t unit) {
   using P = Places<T>;
   auto value = [&](float z) -> uint64_t { return RANK ? 1ull : row.units(z); };
   Place p;
@@ -942,14 +944,20 @@ __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Ro
     const uint64_t e = before + f.before;
     __syncthreads();
     if (threadIdx.x == 0) {
-      s.l.n = 0;
+      s.large.some.l.n = 0;
       s.lo = 0xFFFFFFFFu;
       s.hi = 0;
     }
-    if (e <= unit && unit < e + f.b0 + f.b1) {
-      const uint32_t second = unit >= e + f.b0;
-      s.found = 2 * threadIdx.x + second;
-      s.mass_before = e + (second ? f.b0 : 0);
+    if (e <= unit && unit < e + f.all) {
+      uint64_t start = e;
+#pragma unroll
+      for (uint32_t i = 0; i < f.PER; ++i) {
+        if (start <= unit && unit < start + f.bin[i]) {
+          s.found = f.PER * threadIdx.x + i;
+          s.mass_before = start;
+        }
+        start += f.bin[i];
+      }
     }
     __syncthreads();
     const uint32_t b = s.found;
@@ -967,10 +975,10 @@ __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Ro
         const uint32_t mine = bins.of(z);
         in_pieces += mine < b;
         if (mine == b) {
-          const uint32_t key = score_key(z), at = atomicAdd(&s.l.n, 1u);
+          const uint32_t key = score_key(z), at = atomicAdd(&s.large.some.l.n, 1u);
           kmin = min(kmin, key);
           kmax = max(kmax, key);
-          if (at < CAP) s.l.list[at] = listed(z, c);
+          if (at < CAP<BT>) s.large.some.l.list[at] = listed(z, c);
         }
       }
     });
@@ -981,34 +989,34 @@ __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Ro
       atomicMin(&s.lo, kmin);
       atomicMax(&s.hi, kmax);
     }
-    block_scan<THREADS>(larger, s.wave, &p.larger);  // its barriers publish the list
-    const uint32_t n = s.l.n;
+    block_scan<BT>(larger, s.wave, &p.larger);  // its barriers publish the list
+    const uint32_t n = s.large.some.l.n;
     const float lo = key_score(s.lo), hi = key_score(s.hi);
     if (lo == hi) {  // one value: the place among its equals
       p = Place{hi, Row::quotient(unit - before, value(hi)), n, SKY_INVALID, before, p.larger};
-      if (n == 1) p.column = (uint32_t)s.l.list[0];
+      if (n == 1) p.column = (uint32_t)s.large.some.l.list[0];
       return p;
     }
-    if (n <= CAP) {
-      sort_list<THREADS>(s.l.list, n);
+    if (n <= CAP<BT>) {
+      sort_list<BT>(s.large.some.l.list, n);
       const uint32_t m = lo == low ? n - excess : n, i0 = 2 * threadIdx.x, i1 = i0 + 1;
-      const float z0 = i0 < m ? listed_score(s.l.list[i0]) : 0.0f, z1 = i1 < m ? listed_score(s.l.list[i1]) : 0.0f;
+      const float z0 = i0 < m ? listed_score(s.large.some.l.list[i0]) : 0.0f, z1 = i1 < m ? listed_score(s.large.some.l.list[i1]) : 0.0f;
       const uint64_t v0 = i0 < m ? value(z0) : 0, v1 = i1 < m ? value(z1) : 0;
       uint64_t total;
-      const uint64_t at = before + block_scan<THREADS>(v0 + v1, s.wave, &total);
+      const uint64_t at = before + block_scan<BT>(v0 + v1, s.wave, &total);
       if (at <= unit && unit < at + v0) s.found = i0;
       if (at + v0 <= unit && unit < at + v0 + v1) s.found = i1;
       __syncthreads();
-      const uint64_t entry = s.l.list[s.found];
+      const uint64_t entry = s.large.some.l.list[s.found];
       p.z = listed_score(entry);
       p.column = (uint32_t)entry;
       // its equals in the list: how many come before it, and where the first of them begins
-      const bool equal0 = i0 < n && listed_score(s.l.list[i0]) == p.z, equal1 = i1 < n && listed_score(s.l.list[i1]) == p.z;
-      const bool before0 = i0 ? listed_score(s.l.list[i0 - 1]) != p.z : true;
+      const bool equal0 = i0 < n && listed_score(s.large.some.l.list[i0]) == p.z, equal1 = i1 < n && listed_score(s.large.some.l.list[i1]) == p.z;
+      const bool before0 = i0 ? listed_score(s.large.some.l.list[i0 - 1]) != p.z : true;
       if (equal0 && before0) s.count_before = i0, s.mass_before = at;
       if (equal1 && !equal0) s.count_before = i1, s.mass_before = at + v0;
       uint64_t ties;
-      block_scan<THREADS>((uint64_t)equal0 + (uint64_t)equal1, s.wave, &ties);  // its barriers publish the two above
+      block_scan<BT>((uint64_t)equal0 + (uint64_t)equal1, s.wave, &ties);  // its barriers publish the two above
       p.ties = (uint32_t)ties;
       p.tie = s.found - (uint32_t)s.count_before;
       p.before = s.mass_before;
@@ -1020,8 +1028,8 @@ __device__ __forceinline__ Place locate(const Reader<T>& in, Shared& s, const Ro
   }
 }
 
-template <typename T>
-__device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, const Row& row, const Settings& o, double u, uint32_t most, float zmin,
+template <typename T, int BT>
+__device__ __forceinline__ Result draw_by_bins(const Reader<T, BT>& in, Shared<BT>& s, const Row& row, const Settings& o, double u, uint32_t most, float zmin,
                                                uint32_t there) {
   // What stays is the beginning of the order that ends with `count` entries; entries below `low` weigh nothing or do not belong to it, nor
   // do the last `excess` of value `low`.
@@ -1029,7 +1037,7 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, c
   uint32_t excess = 0, count = there;
   if (o.top_k && o.top_k < there) {
     const Bins bins(row.zmax, zmin);
-    const Filled f = fill_bins<true>(in, s, row, bins, zmin, 0);
+    const Filled<BT> f = fill_bins<true>(in, s, row, bins, zmin, 0);
     const Place p = locate<true>(in, s, row, bins, f, zmin, 0, o.top_k - 1);
     low = p.z;
     count = o.top_k;
@@ -1042,7 +1050,7 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, c
     excess = 0;
   }
   const Bins bins(row.zmax, low);
-  const Filled f = fill_bins<false>(in, s, row, bins, low, excess);
+  const Filled<BT> f = fill_bins<false>(in, s, row, bins, low, excess);
   uint64_t mass = f.total;
   float end = low;
   if (o.top_p < 1.0f) {
@@ -1059,8 +1067,8 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, c
       weighs += row.units(z);
       ++many;
     });
-    block_scan<THREADS>(weighs, s.wave, &all);
-    block_scan<THREADS>(many, s.wave, &all_many);
+    block_scan<BT>(weighs, s.wave, &all);
+    block_scan<BT>(many, s.wave, &all_many);
     if (all_many < count) {
       mass = all;
       count = (uint32_t)all_many;
@@ -1075,13 +1083,13 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T>& in, Shared& s, c
 }
 
 // ---------------------------------------------------------------- the kernel
-template <typename T>
-__device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared& s, const Settings& o, double u) {
+template <typename T, int BT>
+__device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared<BT>& s, const Settings& o, double u) {
   using P = Places<T>;
-  constexpr bool BY_VALUE = sizeof(T) == 2;
-  const bool greedy = o.greedy(), small_k = o.top_k && o.top_k <= SMALL_K, only_min_p = !BY_VALUE && o.min_p > 0.0f && !(o.top_p < 1.0f);
-  const bool few = greedy || small_k || only_min_p;  // few entries can stay
-  Reader<T> in(x, columns);
+  constexpr bool BY_VALUE = sizeof(T) == 2 && BT == THREADS;
+  const bool greedy = o.greedy(), small_k = o.top_k && o.top_k <= SMALL_K<BT>, only_min_p = !BY_VALUE && o.min_p > 0.0f && !(o.top_p < 1.0f);
+  const bool few = o.few(SMALL_K<BT>, !BY_VALUE);
+  Reader<T, BT> in(x, columns);
   uint32_t most, there = 0, above = 0, least = 0xFFFFFFFFu;  // above: the lowest value
   if constexpr (BY_VALUE) {
     auto odd = [&](uint4 w, uint32_t c) {
@@ -1090,7 +1098,7 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared&
         m = max(m, q);
         there += q != 0;
         above += q > P::LOWEST;
-        if (!few && q > P::LOWEST) count_place(s.counters, q);
+        if (!few && q > P::LOWEST) count_place(s.large.counters, q);
       });
       return m;
     };
@@ -1101,16 +1109,16 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared&
     if (few) {
       most = in.first([&](uint4) { regular(Piece<T>::N); }, odd);
     } else {
-      clear_counters(s.counters);
+      clear_counters(s.large.counters);
       __syncthreads();
       most = in.first([&](uint4 p) {
         regular(Piece<T>::N);
-        count_word(s.counters, p.x);
-        count_word(s.counters, p.y);
-        count_word(s.counters, p.z);
-        count_word(s.counters, p.w);
+        count_word(s.large.counters, p.x);
+        count_word(s.large.counters, p.y);
+        count_word(s.large.counters, p.z);
+        count_word(s.large.counters, p.w);
       }, odd);
-      if (in.last > P::LOWEST) count_place(s.counters, in.last);
+      if (in.last > P::LOWEST) count_place(s.large.counters, in.last);
     }
     there += in.last != 0;
     above += in.last > P::LOWEST;
@@ -1143,7 +1151,7 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared&
     __syncthreads();
     most = there = above = 0;
 #pragma unroll
-    for (int i = 0; i < THREADS / 64; ++i) {
+    for (int i = 0; i < BT / 64; ++i) {
       most = max(most, s.wave_most[i]);
       least = min(least, s.wave_least[i]);
       there += s.wave_there[i];
@@ -1158,61 +1166,39 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared&
     return Result{s.place, 1, 0.0};
   }
   const Row row(o.temperature, P::value(most), fraction_bits(columns));
-  if (few || there <= CAP) {
+  if (few || there <= CAP<BT>) {
     uint32_t from = 1;  // places from here on are listed
-    if (there > CAP && small_k) {
+    if (there > CAP<BT> && small_k) {
       // A place that at least top_k of the threads' largest reach, and few more: at least top_k entries reach it.  Up to 128 the
       // largest of four threads do.
       if (threadIdx.x < 64) {
-        uint32_t v[THREADS / 64], lo = 0, hi = most;  // top_k or more reach lo, fewer reach more than hi
-        const bool quads = o.top_k <= THREADS / 8;
+        uint32_t v[BT / 64];
+        const bool quads = o.top_k <= BT / 8;
 #pragma unroll
-        for (int i = 0; i < THREADS / 64; ++i) v[i] = s.most[64 * i + threadIdx.x];
+        for (int i = 0; i < BT / 64; ++i) v[i] = s.most[64 * i + threadIdx.x];
 #pragma unroll
-        for (int i = 0; i < THREADS / 64; i += 4)
+        for (int i = 0; i < BT / 64; i += 4)
           if (quads) v[i / 4] = max(max(v[i], v[i + 1]), max(v[i + 2], v[i + 3]));
-        auto reach = [&](uint32_t place) {
-          uint32_t n = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) n += (uint32_t)__builtin_popcountll(__ballot(v[i] >= place));
-          if (!quads)
-#pragma unroll
-            for (int i = 4; i < THREADS / 64; ++i) n += (uint32_t)__builtin_popcountll(__ballot(v[i] >= place));
-          return n;
-        };
-        uint32_t smallest = v[0];
-#pragma unroll
-        for (int i = 1; i < THREADS / 64; ++i)
-          if (i < 4 || !quads) smallest = min(smallest, v[i]);
-        lo = wave_min_u32(smallest);  // all of them reach it
-        while (lo < hi) {
-          const uint32_t mid = lo + (hi - lo + 1) / 2, n = reach(mid);
-          if (n >= o.top_k) {
-            lo = mid;
-            if (n <= o.top_k + 16) break;
-          } else {
-            hi = mid - 1;
-          }
-        }
+        const uint32_t lo = place_of_rank<BT / 64>(v, quads ? BT / 256 : BT / 64, o.top_k, most);
         if (threadIdx.x == 0) s.place = lo;
       }
       __syncthreads();
       from = max(from, s.place);
     }
-    if (there > CAP && only_min_p) {
+    if (there > CAP<BT> && only_min_p) {
       // the smallest value that may weigh min_p, with a margin for the logarithm
       const double z = (double)row.zmax + row.t * (log((double)o.min_p) - 1e-6) - 1e-6 * fabs((double)row.zmax);
       from = max(from, min(last_failing<T>(most, [&](float v) { return (double)v >= z; }) + 1, most));
     }
     __syncthreads();
-    if (threadIdx.x == 0) s.l.n = 0;
+    if (threadIdx.x == 0) s.large.some.l.n = 0;
     in.from(s, from, [&](uint32_t q, uint32_t c) {
-      const uint32_t at = atomicAdd(&s.l.n, 1u);
-      if (at < CAP) s.l.list[at] = listed(P::value(q), c);
+      const uint32_t at = atomicAdd(&s.large.some.l.n, 1u);
+      if (at < CAP<BT>) s.large.some.l.list[at] = listed(P::value(q), c);
     });
     __syncthreads();
-    const uint32_t n = s.l.n;
-    if (n <= CAP) return draw_list(s.l, n, o, u);
+    const uint32_t n = s.large.some.l.n;
+    if (n <= CAP<BT>) return draw_list(s.large.some.l, n, o, u);
     __syncthreads();  // more than were expected: equal values, or a small min-p
   }
   if constexpr (BY_VALUE) {
@@ -1224,30 +1210,93 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared&
   return draw_by_bins(in, s, row, o, u, most, P::value(least), there);
 }
 
-// A workgroup has a row; `left`: only the rows that draw_short_kernel has left.
+// A workgroup of 1024 threads has a row; `left`: only the rows that draw_short_kernel has left.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void draw_kernel(DrawArgs a, bool left) {
-  __shared__ Shared s;
+  __shared__ Shared<THREADS> s;
   const uint32_t r = blockIdx.x;
   if (left && a.tokens[r * a.tokens_stride] != NOT_DRAWN) return;
   const Settings o(a, r);
-  const Result d = draw_row((const T*)a.logits + r * a.stride, a.columns, s, o, uniform_of(a, r));
+  const Result d = draw_row<T, THREADS>((const T*)a.logits + r * a.stride, a.columns, s, o, uniform_of(a, r));
   if (threadIdx.x == 0) store_result(a, r, d);
 }
 
-// Rows of up to CAP columns are short.  In longer ones draw_short_kernel looks for rows with little in them where there are more rows than
-// a few for each CU; before fewer it would only come on top.
-constexpr uint32_t SPARSE_ROWS = 512;
+// A workgroup of 256 threads has a row, four or more of them a CU: one's loads run beside another's sort.  In longer rows the first
+// columns tell whether most entries are not there; such a row is listed as it is read.  `leave`: rows of which many entries can stay are
+// left to draw_kernel.
+constexpr uint32_t SAMPLE_FROM = 8192;
+template <typename T>
+__global__ __launch_bounds__(SHORT_THREADS, 4) void draw_short_kernel(DrawArgs a, bool leave) {
+  constexpr uint32_t N = Piece<T>::N, STEP = SHORT_THREADS * N, LOADS = 8, LIST = CAP<SHORT_THREADS>;
+  using P = Places<T>;
+  __shared__ Shared<SHORT_THREADS> s;
+  ListShared<SHORT_THREADS>& l = s.large.some.l;
+  const uint32_t r = blockIdx.x, tid = threadIdx.x, columns = a.columns, whole = columns / N * N;
+  const T* const x = (const T*)a.logits + r * a.stride;
+  const Settings o(a, r);
+  const bool few = o.few(SMALL_K<SHORT_THREADS>, true);
+  if (columns > SAMPLE_FROM && !few) {
+    if (tid == 0) l.n = 0;
+    __syncthreads();
+    auto put = [&](uint32_t q, uint32_t c) {
+      if (q) {
+        const uint32_t at = atomicAdd(&l.n, 1u);
+        if (at < LIST) l.list[at] = listed(P::value(q), c);
+      }
+    };
+    auto piece = [&](uint4 w, uint32_t c) {
+      if (piece_max<T>(raw_places<T>(w)) >= P::LOWEST) each<T>(w, c, put);
+    };
+    piece(load_words(x + tid * N), tid * N);
+    __syncthreads();
+    const uint32_t seen = l.n;
+    __syncthreads();
+    if ((uint64_t)seen * columns <= (uint64_t)2 * LIST * STEP) {
+      uint32_t c0 = STEP;
+      for (; c0 + LOADS * STEP <= whole; c0 += LOADS * STEP) {
+        uint4 w[LOADS];
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) w[i] = load_words(x + c0 + i * STEP + tid * N);
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) piece(w[i], c0 + i * STEP + tid * N);
+      }
+      for (uint32_t c = c0 + tid * N; c < whole; c += STEP) piece(load_words(x + c), c);
+      if (whole + tid < columns) put(place_of(x[whole + tid]), whole + tid);
+      __syncthreads();
+      const uint32_t n = l.n;
+      if (n <= LIST) {
+        const Result d = n ? draw_list(l, n, o, uniform_of(a, r)) : nothing_to_draw();
+        if (tid == 0) store_result(a, r, d);
+        return;
+      }
+      __syncthreads();
+    }
+  }
+  if (leave && !few) {
+    if (tid == 0) a.tokens[r * a.tokens_stride] = NOT_DRAWN;
+    return;
+  }
+  const Result d = draw_row<T, SHORT_THREADS>(x, columns, s, o, uniform_of(a, r));
+  if (tid == 0) store_result(a, r, d);
+}
+
+// Which workgroups draw.  One of 256 threads for a row that is short, and for any where there are more rows than CUs: four of them share a
+// CU.  16-bit logits are the exception: a long row of which many entries can stay is drawn from by value, which takes a CU.  (us, 1024 /
+// 256 threads: 2,000 x 8,000 bf16 by top-p 166 / 74, top-k of 50 95 / 23; 1,000 x 20,000 by top-p 105 / 72, 400 x 30,000 48 / 61,
+// 256 x 131,072 45 / 241, 1,000 x 60,000 top-k of 50 56 / 30; fp32 100 x 20,000 by top-p 46 / 39, 600 x 100,000 337 / 248,
+// 40 x 100,003 19 / 43.)
+constexpr uint32_t SHORT_ROW_16 = 20480, SHORT_ROW_32 = 32768, MANY_ROWS = 256;
 template <typename T>
 void launch_draw(const DrawArgs& a, hipStream_t st) {
-  const dim3 grid(a.rows);
-  if (a.columns <= CAP) {
-    hipLaunchKernelGGL((draw_short_kernel<T, false>), grid, dim3(SHORT_THREADS), 0, st, a);
-  } else if (a.rows > SPARSE_ROWS) {
-    hipLaunchKernelGGL((draw_short_kernel<T, true>), grid, dim3(SHORT_THREADS), 0, st, a);
-    hipLaunchKernelGGL(draw_kernel<T>, grid, dim3(THREADS), 0, st, a, true);
+  const dim3 grid(a.rows), few(SHORT_THREADS), all(THREADS);
+  const bool many = a.rows > MANY_ROWS;
+  if (a.columns <= (sizeof(T) == 4 ? SHORT_ROW_32 : SHORT_ROW_16) || (many && sizeof(T) == 4)) {
+    hipLaunchKernelGGL(draw_short_kernel<T>, grid, few, 0, st, a, false);
+  } else if (many) {
+    hipLaunchKernelGGL(draw_short_kernel<T>, grid, few, 0, st, a, true);
+    hipLaunchKernelGGL(draw_kernel<T>, grid, all, 0, st, a, true);
   } else {
-    hipLaunchKernelGGL(draw_kernel<T>, grid, dim3(THREADS), 0, st, a, false);
+    hipLaunchKernelGGL(draw_kernel<T>, grid, all, 0, st, a, false);
   }
 }
 
