@@ -1082,6 +1082,12 @@ __device__ __forceinline__ Result draw_by_bins(const Reader<T, BT>& in, Shared<B
   return r;
 }
 
+// The same out of line, for kernels in which it is an exception and would only take the others' registers.
+template <typename T, int BT>
+__device__ __noinline__ Result draw_by_bins_apart(Reader<T, BT> in, Shared<BT>* s, Row row, Settings o, double u, uint32_t most, float zmin, uint32_t there) {
+  return draw_by_bins(in, *s, row, o, u, most, zmin, there);
+}
+
 // ---------------------------------------------------------------- the kernel
 template <typename T, int BT>
 __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared<BT>& s, const Settings& o, double u) {
@@ -1205,9 +1211,10 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared<
     Result r;
     if (!few && draw_by_value(in, s, row, o, u, most, there, above, &r)) return r;
     __syncthreads();
-    least = P::LOWEST;
+    return draw_by_bins_apart(in, &s, row, o, u, most, P::value(P::LOWEST), there);
+  } else {
+    return draw_by_bins(in, s, row, o, u, most, P::value(least), there);
   }
-  return draw_by_bins(in, s, row, o, u, most, P::value(least), there);
 }
 
 // A workgroup of 1024 threads has a row; `left`: only the rows that draw_short_kernel has left.
