@@ -230,7 +230,8 @@ int sky_sample_session_end(sky_sample_session* s, uint64_t* sampled, double* sec
  *      everything else here runs) and return: they allocate nothing, copy nothing to the host and do not wait, so a stream
  *      that is being captured takes them.  Matrices are row-major in device memory, elements of `dtype`, aligned to the size of
  *      an element; `row_stride` is in elements, 0 stands for as many as a row has.  Nothing behind the last row or the last
- *      column is read or written.  rows == 0 is no error and does nothing.  At most 2^31 - 1 rows and columns. ---- */
+ *      column is read or written.  rows == 0 is no error and does nothing.  At most 2^31 - 1 rows and columns, and what
+ *      each call says (SKY_ERR_LIMIT). ---- */
 enum sky_dtype { SKY_F32 = 0, SKY_F16 = 1, SKY_BF16 = 2 };
 
 /* What is done to logits before a draw, in this order; every part is optional (NULL, zero).  Arrays are device arrays.
@@ -251,7 +252,8 @@ enum sky_dtype { SKY_F32 = 0, SKY_F16 = 1, SKY_BF16 = 2 };
  *                of the paths, or the states of a grammar whose edges lead to ids.  A state that is no vertex, as a walker's that
  *                has stopped, allows nothing.  The graph lives on the current device (SKY_ERR_STATE otherwise).
  * What is not allowed becomes -inf whatever it was, NaN included.  Arithmetic is fp32, rounded to `dtype` once.  `out` is
- * `logits` itself with the same stride, or memory that does not overlap it. */
+ * `logits` itself with the same stride, or memory that does not overlap it.  At most 2^30 columns, and 2^32 - 1 threads: one for 16
+ * columns of a row, 256 for a row that a graph holds. */
 typedef struct sky_logits_rules {
   const uint32_t* history;
   uint64_t history_stride;
@@ -282,16 +284,17 @@ int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, uint32_t col
  *   top_k[r]        only the first top_k of the order stay (0, NULL: all)
  *   top_p[r]        only the shortest beginning of the order whose weight is at least top_p of what top_k left, the first entry in
  *                   any case (NULL, 1 and more, NaN: all)
- *   min_p[r]        only entries of weight min_p and more, the first in any case (NULL, 0: all)
+ *   min_p[r]        only entries of weight min_p and more, the first in any case (NULL, not above 0, NaN: all)
  * The id is the first of what stays whose weights, summed in that order, pass uniforms[r] (in [0, 1)) times their total;
  * uniforms NULL: 53 bits of Philox(philox_seed; first_walker + r, step), a stream that no other call shares.
  * tokens[r * tokens_stride] (stride 0: 1) receives it, so that a column of paths can take it, SKY_INVALID where a row has
  * nothing to draw; logprobs[r] (may be NULL) the logarithm of its probability among what stays (-inf for such a row), kept[r] (may
  * be NULL) how many stay.
  * At most 2^26 columns (SKY_ERR_LIMIT).
- * workspace: memory of the size that sky_logits_draw_workspace gives, aligned to 16 bytes, of which two calls that may run at the same
- * time have one each (a captured graph keeps its own); NULL: every row is drawn from by one workgroup, the same ids, later where
- * there are few rows. */
+ * workspace: sky_logits_draw_workspace says how many bytes a draw of such a matrix can make use of, aligned to 16; two calls that may
+ * run at the same time have one each (a captured graph keeps its own), and NULL is always right: the ids are the same.  Every row
+ * is drawn from within one workgroup's own memory, and the answer is 0 for all matrices; programs that ask need no change where a
+ * later library's draws use some. */
 typedef struct sky_draw_rules {
   const float* temperature;
   const uint32_t* top_k;
@@ -309,12 +312,14 @@ int sky_logits_draw(const void* logits, int dtype, uint32_t rows, uint32_t colum
  * the groups_kept best stay: a group is worth its best expert, or its two best together (group_top2).  ids[r * k + j] receives
  * the j-th best, weights[r * k + j] scale * score, with `renormalise` divided by the sum of the row's k scores; the bias has
  * no part in the weights.  A logit of NaN or -inf closes an expert: it is not chosen, and places that find no open expert receive
- * SKY_INVALID with weight 0; +inf counts as the largest number.  counts[e] (may be NULL) receives how often expert e was chosen
+ * SKY_INVALID with weight 0; +inf counts as the largest number.  A bias of NaN or -inf closes its expert for all rows, one of +inf puts
+ * it before the others.  counts[e] (may be NULL) receives how often expert e was chosen
  * (0 for all when there are no rows).
- * At most 1,024 experts, k of at most 64, at most 64 groups (SKY_ERR_LIMIT).
+ * At most 1,024 experts, k of at most 64, at most 64 groups, at most 2^25 rows (SKY_ERR_LIMIT).
  * The backward call takes the same logits and rules, the ids, and dweights[r * k + j], the gradient with respect to the weights; it
- * writes dlogits, of the logits' dtype, every column of every row.  The choice itself has no gradient, and so the bias has none; closed
- * experts have 0. */
+ * writes dlogits, of the logits' dtype, every column of every row, memory that does not overlap the logits.  The choice itself has no
+ * gradient, and so the bias has none; closed experts have 0.  Ids that are no experts are passed over; those of a row are distinct, as
+ * they were chosen (parts of equal ones are added, in no fixed order). */
 typedef struct sky_route_rules {
   uint32_t k;
   uint32_t groups;

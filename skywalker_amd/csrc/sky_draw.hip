@@ -31,7 +31,8 @@ template <int BT>
 constexpr uint32_t SMALL_K = BT / 2;  // of 1024 threads' largest entries: some 710 entries are as large as the 512th of them
 constexpr uint32_t VALUES = 65536, CHUNK = 256, CHUNKS = VALUES / CHUNK;  // of 16-bit logits; a wavefront takes a chunk, four values a lane
 constexpr int PIECES = 16, AHEAD = 4;  // pieces of 16 bytes that a thread tells apart, and of a load that runs while as many are worked on
-constexpr uint32_t MAX_COLUMNS = 1u << 26;  // a thread counts its elements in 16 bits
+constexpr uint32_t MAX_COLUMNS = 1u << 26;   // weights keep 35 bits, and what an entry's is divided into 27
+constexpr uint32_t SLICE = 1u << 21;         // rows of a launch: fewer than 2^32 threads
 constexpr uint32_t NOT_DRAWN = 0xFFFFFFFEu;  // token of a row that draw_short_kernel leaves to draw_kernel
 
 struct DrawArgs {
@@ -61,7 +62,8 @@ struct Settings {
     top_p = a.top_p ? a.top_p[r] : 1.0f;
     min_p = a.min_p ? a.min_p[r] : 0.0f;
     if (!(top_p < 1.0f)) top_p = 1.0f;
-    if (!(min_p > 0.0f)) min_p = 0.0f;
+    if (min_p > 1.0f) top_k = 1;  // not even the equals of the first entry
+    if (!(min_p > 0.0f && min_p <= 1.0f)) min_p = 0.0f;
   }
   __device__ __forceinline__ bool greedy() const { return !(temperature > 0.0f); }
   // few entries can stay: top-k of up to `small_k`, and where `by_min_p` min-p without top-p
@@ -70,7 +72,7 @@ struct Settings {
   }
 };
 __device__ __forceinline__ double uniform_of(const DrawArgs& a, uint32_t r) {
-  if (a.uniforms) return fmax(a.uniforms[r], 0.0);
+  if (a.uniforms) return fmin(fmax(a.uniforms[r], 0.0), 1.0);
   const u32x4 bits = philox(a.seed, a.first_walker + r, a.step, 0, DOM_LOGITS);
   return ((double)(bits.x >> 5) * 67108864.0 + (double)(bits.y >> 6)) * (1.0 / 9007199254740992.0);
 }
@@ -1342,14 +1344,20 @@ extern "C" int sky_logits_draw(const void* logits, int dtype, uint32_t rows, uin
   for (const auto& x : arrays) SKY_TRY(check_aligned(who, x.name, x.p, x.size));
   if (!rows) return SKY_OK;
   SKY_TRY(ensure_device());
-  const DrawArgs a{logits, row_stride,  columns,      rows, d.temperature, d.top_k,       d.top_p,  d.min_p,
-                   uniforms, philox_seed, first_walker, step, tokens,        tokens_stride ? tokens_stride : 1, logprobs, kept};
+  if (!tokens_stride) tokens_stride = 1;
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == SKY_F32)
-    launch_draw<float>(a, st);
-  else if (dtype == SKY_F16)
-    launch_draw<_Float16>(a, st);
-  else
-    launch_draw<__bf16>(a, st);
-  return check_launch();
+  for (uint32_t r = 0; r < rows; r += SLICE) {
+    auto from = [&](auto* p) { return p ? p + r : p; };
+    const DrawArgs a{(const char*)logits + r * row_stride * dtype_size(dtype), row_stride, columns, std::min(SLICE, rows - r), from(d.temperature),
+                     from(d.top_k), from(d.top_p), from(d.min_p), from(uniforms), philox_seed, first_walker + r, step,
+                     tokens + r * tokens_stride, tokens_stride, from(logprobs), from(kept)};
+    if (dtype == SKY_F32)
+      launch_draw<float>(a, st);
+    else if (dtype == SKY_F16)
+      launch_draw<_Float16>(a, st);
+    else
+      launch_draw<__bf16>(a, st);
+    SKY_TRY(check_launch());
+  }
+  return SKY_OK;
 }

@@ -13,9 +13,8 @@
 // adjust_near_kernel: rows that a graph holds to a vertex's neighbours, up to NEAR of them.  A workgroup has a row: the neighbours
 // go into a hash table in LDS, where history and biases look themselves up, their logits into registers; the row is filled with
 // -inf by a stream of stores, and the neighbours are put in.  Nothing else of the logits is read.  (4,096 rows of 65,536 f16:
-// tiles 234 us, most of it the wait for state, row bounds and neighbours, eight
-// times a row; so 110.)  Rows with more neighbours
-// are done tile by tile by their workgroup.
+// tiles 234 us, most of it the wait for state, row bounds and neighbours, eight times a row; so 109, of which the stores alone are
+// 99.)  Rows with more neighbours are done tile by tile by their workgroup.
 #include "sky_graph.h"
 #include "sky_scores.h"
 
@@ -23,6 +22,7 @@ namespace sky {
 namespace {
 
 constexpr uint32_t COLS = 16;                // columns of a thread
+constexpr uint32_t MAX_COLUMNS = 1u << 30;   // places of tiles are ints, and a tile may end behind the row
 constexpr uint32_t SEEN = 0x80000000u;       // in the history, before history_first
 constexpr uint32_t BIAS_SEARCH_MIN = 2048u;  // from so many biases on a tile looks for its own by bisection (two chains of some 12 loads)
 
@@ -109,7 +109,7 @@ struct Change {
   }
 };
 
-// Tile t of a row, by the workgroup; `lds` holds what tile_words says.
+// Tile t of a row, by the workgroup; `lds`: a word a column for a history, one for biases, a bit for a graph.
 template <typename T>
 __device__ __forceinline__ void adjust_tile(const AdjustArgs& a, uint32_t row, uint32_t t, uint32_t* lds) {
   constexpr int N = Piece<T>::N, NV = COLS / N;
@@ -428,9 +428,20 @@ extern "C" int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, u
   SKY_TRY(check_rows("sky_logits_adjust", "out", out, dtype, rows, columns, &out_stride));
   if (out == logits && out_stride != row_stride) return fail(SKY_ERR_ARG, "sky_logits_adjust: in place with another stride");
   SKY_TRY(check_rules(rules, rows, columns, &a));
+  if (columns > MAX_COLUMNS) return fail(SKY_ERR_LIMIT, "sky_logits_adjust: more than 2^30 columns");
   if (!rows || !columns) return SKY_OK;
+  const size_t size = dtype_size(dtype);
+  const bool aligned = ((uintptr_t)out | out_stride * size) % 16 == 0, near = a.r.graph != nullptr;
+  // counts and biases take 8 bytes of LDS a column: half the tile keeps several workgroups on a CU
+  const uint32_t most = near || (a.r.history && a.r.bias_ids) ? 256 : 512;
+  uint32_t threads = near ? NEAR_THREADS : 64;
+  while (threads < most && threads * COLS < columns) threads *= 2;
+  const uint32_t tile = threads * COLS;
+  a.tiles = (uint32_t)(((uint64_t)columns + (aligned ? 0 : 16 / size - 1) + tile - 1) / tile);
+  const uint64_t grid = near ? rows : (uint64_t)a.tiles * rows;
+  if (grid * threads > 0xFFFFFFFFull) return fail(SKY_ERR_LIMIT, "sky_logits_adjust: more than 2^32 - 1 threads, one for 16 columns or 256 for a row by a graph");
   SKY_TRY(ensure_device());
-  if (a.r.graph) {
+  if (near) {
     int dev = 0;
     SKY_HIP(hipGetDevice(&dev));
     if (dev != a.r.graph->device)
@@ -445,37 +456,14 @@ extern "C" int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, u
   a.stride = row_stride;
   a.out_stride = out_stride;
   a.columns = columns;
-  const size_t size = dtype_size(dtype);
-  const bool aligned = ((uintptr_t)out | out_stride * size) % 16 == 0;
-  const hipStream_t st = (hipStream_t)stream;
-  auto tiles = [&](uint32_t tile) { return (uint32_t)(((uint64_t)columns + (aligned ? 0 : 16 / size - 1) + tile - 1) / tile); };
-  if (a.xadj) {
-    const uint32_t tile = NEAR_THREADS * COLS;
-    a.tiles = tiles(tile);
-    const bool tables = a.r.history || a.r.bias_ids;
-    const size_t lds = std::max<size_t>(tables ? 3 * SLOTS : 0, (a.r.history ? tile : 0u) + (a.r.bias_ids ? tile : 0u) + tile / 32) * 4;
-    if (dtype == SKY_F32)
-      hipLaunchKernelGGL(adjust_near_kernel<float>, dim3(rows), dim3(NEAR_THREADS), lds, st, a);
-    else if (dtype == SKY_F16)
-      hipLaunchKernelGGL(adjust_near_kernel<_Float16>, dim3(rows), dim3(NEAR_THREADS), lds, st, a);
-    else
-      hipLaunchKernelGGL(adjust_near_kernel<__bf16>, dim3(rows), dim3(NEAR_THREADS), lds, st, a);
-    return check_launch();
-  }
-  // counts and biases take 8 bytes of LDS a column: half the tile keeps several workgroups on a CU
-  const uint32_t most = a.r.history && a.r.bias_ids ? 256 : 512;
-  uint32_t threads = 64;
-  while (threads < most && threads * COLS < columns) threads *= 2;
-  const uint32_t tile = threads * COLS;
-  a.tiles = tiles(tile);
-  if ((uint64_t)a.tiles * rows > 0x7FFFFFFFull) return fail(SKY_ERR_LIMIT, "sky_logits_adjust: too many tiles");
-  const size_t lds = ((a.r.history ? tile : 0u) + (a.r.bias_ids ? tile : 0u)) * 4;
-  const dim3 grid(a.tiles * rows), block(threads);
+  const uint32_t arrays = (a.r.history ? tile : 0u) + (a.r.bias_ids ? tile : 0u);
+  const uint32_t lds = !near ? arrays : std::max(a.r.history || a.r.bias_ids ? 3 * SLOTS : 0u, arrays + tile / 32);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), lds * 4, (hipStream_t)stream, a); };
   if (dtype == SKY_F32)
-    hipLaunchKernelGGL(adjust_kernel<float>, grid, block, lds, st, a);
+    near ? launch(adjust_near_kernel<float>) : launch(adjust_kernel<float>);
   else if (dtype == SKY_F16)
-    hipLaunchKernelGGL(adjust_kernel<_Float16>, grid, block, lds, st, a);
+    near ? launch(adjust_near_kernel<_Float16>) : launch(adjust_kernel<_Float16>);
   else
-    hipLaunchKernelGGL(adjust_kernel<__bf16>, grid, block, lds, st, a);
+    near ? launch(adjust_near_kernel<__bf16>) : launch(adjust_kernel<__bf16>);
   return check_launch();
 }

@@ -19,6 +19,7 @@ namespace sky {
 namespace {
 
 constexpr uint32_t MAX_EXPERTS = 1024, MAX_K = 64, MAX_GROUPS = 64;
+constexpr uint32_t MAX_ROWS = 1u << 25;  // a launch has fewer than 2^32 threads, 64 for a row at most
 constexpr int ROUTE_WAVES = 4;  // of a workgroup
 
 struct RouteArgs {
@@ -69,6 +70,14 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
   return v;
 }
 __device__ __forceinline__ bool open_expert(float x) { return x > -__builtin_inff(); }
+// Whether a bias of the wavefront's is infinite or NaN: the bound of the fp32 choices does not hold then.
+template <int PER>
+__device__ __forceinline__ bool some_not_finite(const float (&bias)[PER]) {
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) odd |= !(fabsf(bias[i]) < __builtin_inff());
+  return __ballot(odd) != 0;
+}
 // e^x of x <= 0, to some 1e-14: the series of e^f on |f| <= ln(2) / 2 through degree 11
 __device__ __forceinline__ double exp_negative(double x) {
   const double t = fmax(x * 1.44269504088896340736, -1000.0), n = rint(t), f = (t - n) * 0.69314718055994530942;
@@ -116,7 +125,8 @@ __device__ __forceinline__ uint32_t choose_exactly(const T* x, const RouteArgs& 
     key[i] = 0;
     if (open_expert(z[i])) {
       const double score = by_logit ? (double)z[i] : a.r.sigmoid ? 1.0 / (1.0 + exp(-(double)z[i])) : exp((double)z[i] - (double)zmax) / sum;
-      key[i] = double_key(score + (a.r.bias ? (double)a.r.bias[e] : 0.0));
+      const double choice = score + (a.r.bias ? (double)a.r.bias[e] : 0.0);
+      if (choice > -__builtin_inf()) key[i] = double_key(choice);
     }
   }
   if (a.r.groups > 1 && a.r.groups_kept < a.r.groups) {
@@ -273,6 +283,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
   float bias[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) bias[i] = a.r.bias && sub * PER + i < E ? a.r.bias[sub * PER + i] : 0.0f;
+  const bool odd = some_not_finite(bias);
   s.id[lane] = SKY_INVALID;
   for (uint32_t t = 0; t < turns; ++t) {
     const uint32_t n = 4 * t + quarter;  // of the wavefront's rows
@@ -339,7 +350,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
       }
       near = (a.r.sigmoid ? 0x1p-20f : 0x1p-18f * most) + 0x1p-22f * key_score(max16(score_key(size_of_choice)));
     }
-    bool doubt = false;  // of this lane
+    bool doubt = odd;  // of this lane
     if (grouped) {
       uint32_t best = 0, second = 0, owner;  // owner: the lane that speaks for this lane's experts
       if (whole_lanes) {
@@ -434,7 +445,8 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
       }
     }
     __builtin_amdgcn_wave_barrier();
-    if (!by_logit && sub < k && sub < listed && !(s.best[quarter][sub] - s.best[quarter][sub + 1] > near)) {
+    // (best[listed] is -inf, further than any bound from a finite number: place[listed], which is not set, is then not looked at)
+    if (!by_logit && !odd && sub < k && sub < listed && !(s.best[quarter][sub] - s.best[quarter][sub + 1] > near)) {
       // alike, the same logit and bias, they stand as they are
       const uint32_t e = s.place[quarter][sub], f = s.place[quarter][sub + 1];
       doubt |= !((float)x[e] == (float)x[f] && (!a.r.bias || a.r.bias[e] == a.r.bias[f]));
@@ -476,6 +488,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
   float bias[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) bias[i] = a.r.bias && lane * PER + i < E ? a.r.bias[lane * PER + i] : 0.0f;
+  const bool odd = some_not_finite(bias);
   uint32_t id = SKY_INVALID;
   double my_sum = 0.0;
   float my_max = 0.0f;
@@ -545,7 +558,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
       size_of_choice = key_score(wave_top(score_key(size_of_choice)));
       near = (a.r.sigmoid ? 0x1p-20f : 0x1p-18f * most) + 0x1p-22f * size_of_choice;
     }
-    bool exact = true;  // the choice so far
+    bool exact = !odd;  // the choice so far
     if (grouped) {
       uint32_t best = 0, second = 0;
       uint32_t owner = lane;  // of which group this lane tells the worth, and the first lane of its own group's lanes
@@ -794,7 +807,7 @@ int check_route(const char* who, uint32_t rows, uint32_t experts, const sky_rout
   if (r->k > r->groups_kept * (experts / r->groups)) return arg("the kept groups have fewer than k experts");
   if (!(r->scale - r->scale == 0.0f)) return arg("scale is not a finite number");
   SKY_TRY(check_aligned(who, "bias", r->bias, 4));
-  if (rows > 0x7FFFFFFFu / (uint32_t)ROUTE_WAVES * ROUTE_WAVES) return fail(SKY_ERR_LIMIT, std::string(who) + ": too many rows");
+  if (rows > MAX_ROWS) return fail(SKY_ERR_LIMIT, std::string(who) + ": more than 2^25 rows");
   return SKY_OK;
 }
 

@@ -295,6 +295,42 @@ def test_draw_of_many_rows(capi, orc, dtype):
              min_p=rng.choice([0.0, 0.01], 700), u=rng.random(700), workspace=True)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("columns", [700, 5000, 40007])
+def test_draw_by_a_min_p_above_one_leaves_the_first_entry(capi, orc, dtype, columns):
+    rng = np.random.default_rng(columns)
+    x = rng.integers(-3, 4, (4, columns)).astype(np.float32)  # many are as large as the largest
+    for m in (1.0, 1.5):
+        for p in (1.0, 0.9):
+            run_draw(capi, orc, x, dtype, min_p=np.full(4, m), top_p=np.full(4, p), u=rng.random(4))
+
+
+@pytest.mark.parametrize("dtype,columns", [("f32", 33001), ("f16", 20611), ("bf16", 20611)])
+def test_draw_of_many_long_rows(capi, orc, dtype, columns):
+    # more rows than CUs, some of which most entries are missing from, some to be drawn from few entries, some from all
+    rng = np.random.default_rng(columns)
+    n = 270
+    x = rng.normal(0, 2, (n, columns)).astype(np.float32)
+    x[::5][rng.random(x[::5].shape) < 0.995] = -INF
+    x[1::9, 3000:] = -INF  # as full as can be where the kernel looks first, empty behind
+    x[2::9, :3000] = -INF
+    x[7] = -INF
+    run_draw(capi, orc, x, dtype, pad=1, t=rng.choice([0.0, 0.4, 1.0, 2.0], n), top_k=rng.choice([0, 0, 20, 200, 700], n),
+             top_p=rng.choice([1.0, 0.9, 0.5], n), min_p=rng.choice([0.0, 0.0, 0.02], n), u=rng.random(n))
+
+
+def test_draw_of_more_rows_than_a_launch_has(capi):
+    rows = (1 << 21) + 5
+    x = np.random.default_rng(13).normal(0, 2, (rows, 2)).astype(np.float16)
+    m, tokens, kept = dev(capi, x, np.float16), capi.DeviceArray(rows, np.uint32), capi.DeviceArray(rows, np.uint32)
+    capi.logits_draw(m, capi.F16, rows, 2, capi.DrawRules(temperature=dev(capi, np.zeros(rows), np.float32)), tokens, kept=kept)
+    assert np.array_equal(tokens.to_host(), (x[:, 1] > x[:, 0]).astype(np.uint32)) and (kept.to_host() == 1).all()
+    capi.logits_draw(m, capi.F16, rows, 2, None, tokens, seed=5, first_walker=7)
+    last, end = dev(capi, x[-9:], np.float16), capi.DeviceArray(9, np.uint32)
+    capi.logits_draw(last, capi.F16, 9, 2, None, end, seed=5, first_walker=7 + rows - 9)
+    assert np.array_equal(tokens.to_host()[-9:], end.to_host())
+
+
 # ------------------------------------------------------------------------------------------------ route
 def run_route(capi, x, dtype, k, pad=0, lead=0, counts=True, **kw):
     rows, E = x.shape
@@ -390,6 +426,20 @@ def test_route_of_equal_groups_and_equal_choices(capi, sigmoid):
             for groups, kept, k in ((8, 3, 7), (1, 1, 16), (16, 5, 16), (32, 20, 9), (8, 4, 33)):
                 run_route(capi, x, "f32", k, sigmoid=sigmoid, bias=b, groups=groups, kept=kept, top2=top2)
                 run_route(capi, x[:, :96], "bf16", min(k, 15), sigmoid=sigmoid, bias=None if b is None else b[:96], groups=groups, kept=max(kept, -(-min(k, 15) // (96 // groups))), top2=top2, renormalise=False)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("E,groups,kept,k", [(24, 1, 1, 5), (256, 8, 3, 8), (256, 32, 9, 8), (600, 1, 1, 20)])
+def test_route_by_biases_that_are_no_finite_numbers(capi, sigmoid, E, groups, kept, k):
+    # -inf and NaN close an expert, +inf puts it first
+    rng = np.random.default_rng(E + groups)
+    x = rng.normal(0, 2, (19, E)).astype(np.float32)
+    bias = rng.uniform(-0.2, 0.2, E).astype(np.float32)
+    for odd in ((-INF,), (np.nan,), (INF,), (-INF, np.nan, INF)):
+        b = bias.copy()
+        b[rng.permutation(E)[: E // 3]] = np.resize(np.array(odd, np.float32), E // 3)
+        for top2 in (False, True):
+            run_route(capi, x, "f32", k, sigmoid=sigmoid, bias=b, groups=groups, kept=kept, top2=top2)
 
 
 def test_route_of_a_long_batch(capi):

@@ -106,6 +106,16 @@ def test_route_refusals(capi):
     refused(capi, ARG, "null", capi.route_topk_backward, x, capi.F32, 1, 8, rules(1), i, w, None)
 
 
+def test_sizes_beyond_a_launch_are_refused(capi):
+    x, y = Fake(), Fake(8192)
+    refused(capi, LIMIT, "2^30", capi.logits_adjust, x, capi.BF16, 1, (1 << 30) + 1, None, y)
+    refused(capi, LIMIT, "threads", capi.logits_adjust, x, capi.BF16, 1 << 23, 8192, None, y)
+    refused(capi, LIMIT, "threads", capi.logits_adjust, x, capi.BF16, 1 << 26, 50, None, y)
+    refused(capi, LIMIT, "2^26", capi.logits_draw, x, capi.F16, 1, (1 << 26) + 1, None, y)
+    refused(capi, LIMIT, "2^25", capi.route_topk, x, capi.F32, (1 << 25) + 1, 8, capi.RouteRules(1), y, Fake(16384))
+    refused(capi, LIMIT, "2^25", capi.route_topk_backward, x, capi.F32, (1 << 25) + 1, 8, capi.RouteRules(1), y, Fake(16384), Fake(32768))
+
+
 def test_no_rows_are_no_work(capi):
     # no GPU is asked for, and no pointer needed
     capi.logits_adjust(None, capi.F32, 0, 8, None, None)
