@@ -291,10 +291,9 @@ int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, uint32_t col
  * nothing to draw; logprobs[r] (may be NULL) the logarithm of its probability among what stays (-inf for such a row), kept[r] (may
  * be NULL) how many stay.
  * At most 2^26 columns (SKY_ERR_LIMIT).
- * workspace: sky_logits_draw_workspace says how many bytes a draw of such a matrix can make use of, aligned to 16; two calls that may
- * run at the same time have one each (a captured graph keeps its own), and NULL is always right: the ids are the same.  Every row
- * is drawn from within one workgroup's own memory, and the answer is 0 for all matrices; programs that ask need no change where a
- * later library's draws use some. */
+ * workspace: sky_logits_draw_workspace says how many bytes a draw of such a matrix can make use of (0: none), aligned to 16; nothing need
+ * be in them, two calls that may run at the same time have one workspace each, and a captured graph keeps its own.  With it several
+ * workgroups share each of a few long fp32 rows; NULL: every row is drawn from by one workgroup, the same ids, later. */
 typedef struct sky_draw_rules {
   const float* temperature;
   const uint32_t* top_k;

@@ -281,8 +281,9 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* waves, uint
   return before + inclusive - v;
 }
 
-// list[0..m) into the order.  Up to an entry a thread: every entry's rank is counted (no barrier between the steps); longer lists
-// by a bitonic network over the next power of two.  (Lists of 64: 1.2 us less than by the network.)
+// list[0..m) into the order.  Up to an entry for two threads: every entry's rank is counted (no barrier between the steps); longer lists
+// by a bitonic network over the next power of two.  (us, network alone / so: 2,000 x 8,000 bf16 by top-k of 50 32 / 23, 8 x 131,072 fp32
+// by top-k of 120 25 / 22, of 400 34 / 34.)
 template <int BT>
 __device__ __forceinline__ void sort_list(uint64_t* list, uint32_t m) {
   if (m <= BT / 2) {
@@ -1090,6 +1091,24 @@ __device__ __noinline__ Result draw_by_bins_apart(Reader<T, BT> in, Shared<BT>* 
   return draw_by_bins(in, *s, row, o, u, most, zmin, there);
 }
 
+// s.place: a place that at least k of the threads' largest (s.most) reach, and few more, so that at least k entries reach it.  Up to
+// BT / 8 the largest of four threads do.  Its barrier publishes it.
+template <int BT>
+__device__ __forceinline__ void place_for_rank(Shared<BT>& s, uint32_t k, uint32_t most) {
+  if (threadIdx.x < 64) {
+    uint32_t v[BT / 64];
+    const bool quads = k <= BT / 8;
+#pragma unroll
+    for (int i = 0; i < BT / 64; ++i) v[i] = s.most[64 * i + threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < BT / 64; i += 4)
+      if (quads) v[i / 4] = max(max(v[i], v[i + 1]), max(v[i + 2], v[i + 3]));
+    const uint32_t lo = place_of_rank<BT / 64>(v, quads ? BT / 256 : BT / 64, k, most);
+    if (threadIdx.x == 0) s.place = lo;
+  }
+  __syncthreads();
+}
+
 // ---------------------------------------------------------------- the kernel
 template <typename T, int BT>
 __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared<BT>& s, const Settings& o, double u) {
@@ -1177,20 +1196,7 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared<
   if (few || there <= CAP<BT>) {
     uint32_t from = 1;  // places from here on are listed
     if (there > CAP<BT> && small_k) {
-      // A place that at least top_k of the threads' largest reach, and few more: at least top_k entries reach it.  Up to 128 the
-      // largest of four threads do.
-      if (threadIdx.x < 64) {
-        uint32_t v[BT / 64];
-        const bool quads = o.top_k <= BT / 8;
-#pragma unroll
-        for (int i = 0; i < BT / 64; ++i) v[i] = s.most[64 * i + threadIdx.x];
-#pragma unroll
-        for (int i = 0; i < BT / 64; i += 4)
-          if (quads) v[i / 4] = max(max(v[i], v[i + 1]), max(v[i + 2], v[i + 3]));
-        const uint32_t lo = place_of_rank<BT / 64>(v, quads ? BT / 256 : BT / 64, o.top_k, most);
-        if (threadIdx.x == 0) s.place = lo;
-      }
-      __syncthreads();
+      place_for_rank<BT>(s, o.top_k, most);
       from = max(from, s.place);
     }
     if (there > CAP<BT> && only_min_p) {
@@ -1219,14 +1225,410 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared<
   }
 }
 
+// ---------------------------------------------------------------- a few long rows, in parts
+// A workgroup alone takes a row of fp32 logits at what a CU reads, three or four times, and where there are few rows most CUs have
+// nothing to do.  With a workspace `parts` workgroups share a row, in kernels that follow one another:
+//   parts_kernel    each part's largest and smallest place and how many entries are there; of rows that are drawn from by top-k of up to
+//                   PART_K or greedily the part's k best, in the order
+//   fill_kernel     the mass and the number of the entries of every bin, as draw_by_bins has them
+//   collect_kernel  the entries of the bin in which top-p or min-p ends the row, and of those bins in which the drawn unit lies for any end in that
+//                   bin (next to always one or two)
+//   draw_kernel     the draw from these
+// All sums are whole numbers in the same units, so that the ids are the same.  What does not fit (top-k above PART_K, min-p without top-p, rows with
+// next to nothing in them, lists that run over) is drawn from by draw_kernel alone.
+constexpr uint32_t PART_K = SMALL_K<SHORT_THREADS>, MAX_PARTS = 16, MANY_EQUAL = 0xFFFFFFFFu;
+struct RowSpace {  // of a row in the workspace
+  uint64_t bin[BINS];
+  uint64_t list[CAP<THREADS>];              // what collect_kernel found
+  uint64_t part_list[MAX_PARTS][PART_K];
+  uint32_t count[BINS];
+  uint32_t most[MAX_PARTS], least[MAX_PARTS], there[MAX_PARTS], part_count[MAX_PARTS];
+  uint32_t n, unused[3];                    // entries of `list`
+};
+struct Parts {
+  RowSpace* space;
+  uint32_t parts, span;
+};
+// What the parts have found of a row that is neither greedy nor to be drawn from by a small top-k.
+struct Whole {
+  uint32_t most, least, there;
+  __device__ __forceinline__ Whole(const RowSpace& w, uint32_t parts) {
+    const uint32_t lane = threadIdx.x & 63;
+    const bool in = lane < parts;
+    most = wave_max_u32(in ? w.most[lane] : 0);
+    least = wave_min_u32(in ? w.least[lane] : 0xFFFFFFFFu);
+    there = (uint32_t)__shfl((int)group_scan_u32<64>(in ? w.there[lane] : 0), 63, 64);
+  }
+};
+__device__ __forceinline__ bool drawn_in_parts(const Settings& o, const Whole& w) {
+  return w.there > CAP<THREADS> && !(o.top_k && o.top_k < w.there) && !(o.min_p > 0.0f && !(o.top_p < 1.0f));
+}
+__device__ __forceinline__ Bins bins_of(const Row& row, const Whole& w) {
+  const float cut = (float)fmax((double)row.zmax - NO_MASS * row.t, -3.402823466e38);
+  return Bins(row.zmax, fmaxf(key_score(w.least), cut));
+}
+// The smallest value that weighs min_p, by a wavefront: six bits of its place at a time.
+__device__ __forceinline__ float least_of_min_p(const Row& row, float min_p, uint32_t most) {
+  using P = Places<float>;
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t lo = 0;  // the largest place known to weigh less
+#pragma unroll 1
+  for (int shift = 26; shift > -6; shift -= 6) {
+    const int by = max(shift, 0);
+    const uint32_t q = lo | lane << by;
+    const bool fails = q <= most && (shift >= 0 || lane < 4) && (q < P::LOWEST || !(row.weight(P::value(q)) >= (double)min_p));
+    lo |= (63u - (uint32_t)__builtin_clzll(__ballot(fails) | 1ull)) << by;
+  }
+  return P::value(min(lo + 1, most));
+}
+// Where the row ends and where the drawn unit may lie, from the bins, BINS / BT a thread: by every thread.
+template <int BT>
+struct Ends {
+  static constexpr uint32_t PER = BINS / BT;
+  uint64_t mine[PER], before, total;  // the thread's bins, and what lies before them
+  uint32_t p, m, end;                 // bins in which top-p and min-p end, the first of them; BINS: none
+  uint64_t need, end_before, end_mass;
+  template <typename F>
+  __device__ __forceinline__ void each_own(F f) const {
+    uint64_t b = before;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) {
+      f(PER * threadIdx.x + i, b, mine[i]);
+      b += mine[i];
+    }
+  }
+  // the bin that holds a unit of mass; `at`: what lies before it
+  __device__ __forceinline__ uint32_t bin_of(Shared<BT>& s, uint64_t unit, uint64_t* at) const {
+    __syncthreads();
+    each_own([&](uint32_t b, uint64_t start, uint64_t size) {
+      if (start <= unit && unit < start + size) {
+        s.found = b;
+        s.mass_before = start;
+      }
+    });
+    __syncthreads();
+    *at = s.mass_before;
+    return s.found;
+  }
+  __device__ __forceinline__ Ends(Shared<BT>& s, const RowSpace& w, const Settings& o, const Bins& bins, float z_least) {
+    uint64_t sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) sum += mine[i] = w.bin[PER * threadIdx.x + i];
+    before = block_scan<BT>(sum, s.wave, &total);
+    p = m = BINS;
+    need = 0;
+    if (o.top_p < 1.0f) {
+      need = Row::needed(o.top_p, total);
+      p = bin_of(s, need - 1, &end_before);
+    }
+    if (o.min_p > 0.0f && bins.has(z_least)) m = bins.of(z_least);
+    end = min(p, m);
+    end_before = 0;
+    end_mass = total;
+    if (end < BINS) {
+      __syncthreads();
+      each_own([&](uint32_t b, uint64_t start, uint64_t size) {
+        if (b == end) {
+          s.mass_before = start;
+          s.count_before = size;
+        }
+      });
+      __syncthreads();
+      end_before = s.mass_before;
+      end_mass = s.count_before;
+    }
+  }
+};
+
+__global__ __launch_bounds__(SHORT_THREADS, 4) void parts_kernel(DrawArgs a, Parts p) {
+  constexpr int BT = SHORT_THREADS;
+  using T = float;
+  using P = Places<T>;
+  __shared__ Shared<BT> s;
+  ListShared<BT>& l = s.large.some.l;
+  const uint32_t r = blockIdx.x / p.parts, part = blockIdx.x % p.parts, start = part * p.span, tid = threadIdx.x;
+  RowSpace& w = p.space[r];
+  const Settings o(a, r);
+  const bool few = o.few(PART_K, false);
+  Reader<T, BT> in((const T*)a.logits + r * a.stride + start, min(p.span, a.columns - start));
+  if (!few) {  // what the next kernels add to
+    for (uint32_t i = part * BT + tid; i < BINS; i += p.parts * BT) {
+      w.bin[i] = 0;
+      w.count[i] = 0;
+    }
+    if (part == 0 && tid == 0) w.n = 0;
+  }
+  uint32_t there = 0, least = 0xFFFFFFFFu;
+  uint32_t most = in.first([&](uint4 q) {
+    there += Piece<T>::N;
+    least = min(least, piece_min<T>(q));
+  }, [&](uint4 v, uint32_t c) {
+    uint32_t m = 0;
+    each<T>(v, c, [&](uint32_t q, uint32_t) {
+      m = max(m, q);
+      there += q != 0;
+      least = q ? min(least, q) : least;
+    });
+    return m;
+  });
+  there += in.last != 0;
+  least = in.last ? min(least, in.last) : least;
+  s.most[tid] = most;
+  most = wave_max_u32(most);
+  least = wave_min_u32(least);
+  there = group_scan_u32<64>(there);
+  if ((tid & 63) == 63) {
+    s.wave_most[tid >> 6] = most;
+    s.wave_least[tid >> 6] = least;
+    s.wave_there[tid >> 6] = there;
+  }
+  if (tid == 0) l.n = 0;
+  __syncthreads();
+  most = there = 0;
+#pragma unroll
+  for (int i = 0; i < BT / 64; ++i) {
+    most = max(most, s.wave_most[i]);
+    least = min(least, s.wave_least[i]);
+    there += s.wave_there[i];
+  }
+  if (!few) {
+    if (tid == 0) {
+      w.most[part] = most;
+      w.least[part] = least;
+      w.there[part] = there;
+    }
+    return;
+  }
+  const uint32_t k = o.greedy() ? 1 : o.top_k;
+  uint32_t from = 1;
+  if (there > CAP<BT>) {
+    place_for_rank<BT>(s, k, most);
+    from = max(from, s.place);
+  }
+  if (there)
+    in.from(s, from, [&](uint32_t q, uint32_t c) {
+      const uint32_t at = atomicAdd(&l.n, 1u);
+      if (at < CAP<BT>) l.list[at] = listed(P::value(q), start + c);
+    });
+  __syncthreads();
+  const uint32_t n = l.n;
+  if (n > CAP<BT>) {
+    if (tid == 0) w.part_count[part] = MANY_EQUAL;
+    return;
+  }
+  sort_list<BT>(l.list, n);
+  const uint32_t m = min(n, k);
+  if (tid == 0) w.part_count[part] = m;
+  if (tid < m) w.part_list[part][tid] = l.list[tid];
+}
+
+// f(value, column) for the entries of a part from `low` on.
+template <typename F>
+__device__ __forceinline__ void each_of_part(const Reader<float, SHORT_THREADS>& in, float low, F f) {
+  using P = Places<float>;
+  auto one = [&](uint32_t bits, uint32_t c) {
+    const uint32_t q = place_of_bits<float>(bits);
+    const float z = P::value(q);
+    if (q && z >= low) f(z, c);
+  };
+  in.stream([&](uint4 v, uint32_t c) {
+    one(v.x, c);
+    one(v.y, c + 1);
+    one(v.z, c + 2);
+    one(v.w, c + 3);
+  });
+  if (in.whole + threadIdx.x < in.columns) one(__float_as_uint(in.x[in.whole + threadIdx.x]), in.whole + threadIdx.x);
+}
+
+__global__ __launch_bounds__(SHORT_THREADS, 4) void fill_kernel(DrawArgs a, Parts p) {
+  __shared__ uint64_t bin[BINS];
+  __shared__ uint32_t count[BINS];
+  const uint32_t r = blockIdx.x / p.parts, start = blockIdx.x % p.parts * p.span;
+  RowSpace& w = p.space[r];
+  const Settings o(a, r);
+  if (o.few(PART_K, false)) return;
+  const Whole whole(w, p.parts);
+  if (!drawn_in_parts(o, whole)) return;
+  const Row row(o.temperature, key_score(whole.most), fraction_bits(a.columns));
+  const Bins bins = bins_of(row, whole);
+  for (uint32_t i = threadIdx.x; i < BINS; i += SHORT_THREADS) {
+    bin[i] = 0;
+    count[i] = 0;
+  }
+  __syncthreads();
+  const Reader<float, SHORT_THREADS> in((const float*)a.logits + r * a.stride + start, min(p.span, a.columns - start));
+  each_of_part(in, bins.low, [&](float z, uint32_t) {
+    const uint32_t b = bins.of(z);
+    atomicAdd((unsigned long long*)&bin[b], (unsigned long long)row.units(z));
+    atomicAdd(&count[b], 1u);
+  });
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < BINS; i += SHORT_THREADS)
+    if (count[i]) {
+      atomicAdd((unsigned long long*)&w.bin[i], (unsigned long long)bin[i]);
+      atomicAdd(&w.count[i], count[i]);
+    }
+}
+
+__global__ __launch_bounds__(SHORT_THREADS, 4) void collect_kernel(DrawArgs a, Parts p) {
+  __shared__ Shared<SHORT_THREADS> s;
+  const uint32_t r = blockIdx.x / p.parts, start = blockIdx.x % p.parts * p.span;
+  RowSpace& w = p.space[r];
+  const Settings o(a, r);
+  if (o.few(PART_K, false)) return;
+  const Whole whole(w, p.parts);
+  if (!drawn_in_parts(o, whole)) return;
+  const Row row(o.temperature, key_score(whole.most), fraction_bits(a.columns));
+  const Bins bins = bins_of(row, whole);
+  const float z_least = o.min_p > 0.0f ? least_of_min_p(row, o.min_p, whole.most) : 0.0f;
+  const Ends<SHORT_THREADS> ends(s, w, o, bins, z_least);
+  const double u = uniform_of(a, r);
+  uint64_t before;
+  const uint64_t least_mass = ends.end < BINS ? max(ends.end_before, (uint64_t)1) : ends.total;
+  const uint32_t first = ends.bin_of(s, Row::drawn(u, least_mass), &before);
+  const uint32_t last = ends.bin_of(s, Row::drawn(u, ends.end_before + ends.end_mass), &before);
+  const Reader<float, SHORT_THREADS> in((const float*)a.logits + r * a.stride + start, min(p.span, a.columns - start));
+  each_of_part(in, bins.low, [&](float z, uint32_t c) {
+    const uint32_t b = bins.of(z);
+    if (b == ends.end || (b >= first && b <= last)) {
+      const uint32_t at = atomicAdd(&w.n, 1u);
+      if (at < CAP<THREADS>) w.list[at] = listed(z, start + c);
+    }
+  });
+}
+
+// The draw from what the parts have left; false: it is none of theirs.
+__device__ __forceinline__ bool draw_collected(Shared<THREADS>& s, const RowSpace& w, uint32_t parts, uint32_t columns, const Settings& o, double u, Result* d) {
+  constexpr uint32_t PER = BINS / THREADS;
+  static_assert(PER == 2 && CAP<THREADS> == 2 * THREADS, "two bins and two entries a thread");
+  const Whole whole(w, parts);
+  const uint32_t n = w.n;
+  if (!drawn_in_parts(o, whole) || n > CAP<THREADS>) return false;
+  const Row row(o.temperature, key_score(whole.most), fraction_bits(columns));
+  const Bins bins = bins_of(row, whole);
+  uint64_t* const list = s.large.some.l.list;
+  for (uint32_t i = threadIdx.x; i < n; i += THREADS) list[i] = w.list[i];
+  const float z_least = o.min_p > 0.0f ? least_of_min_p(row, o.min_p, whole.most) : 0.0f;
+  const Ends<THREADS> ends(s, w, o, bins, z_least);
+  // entries in the bins before the one that ends the row
+  uint64_t mine = 0, larger;
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) mine += PER * threadIdx.x + i < ends.end ? w.count[PER * threadIdx.x + i] : 0;
+  block_scan<THREADS>(mine, s.wave, &larger);  // its barriers publish the list
+  sort_list<THREADS>(list, n);
+  uint32_t bin[2], many = 0;
+  uint64_t mass[2], weighs = 0, sum;
+  float z[2];
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) {
+    const uint32_t at = 2 * threadIdx.x + i;
+    z[i] = at < n ? listed_score(list[at]) : 0.0f;
+    bin[i] = at < n ? bins.of(z[i]) : BINS + 1;
+    mass[i] = at < n ? row.units(z[i]) : 0;
+    if (bin[i] == ends.m && z[i] >= z_least) {
+      ++many;
+      weighs += mass[i];
+    }
+  }
+  const uint64_t before = block_scan<THREADS>(mass[0] + mass[1], s.wave, &sum), own[2] = {before, before + mass[0]};
+  // f(entry, what lies before it in its bin) for the entries of bin b
+  auto in_bin = [&](uint32_t b, auto f) {
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      const uint32_t at = 2 * threadIdx.x + i;
+      if (bin[i] == b && (at == 0 || bins.of(listed_score(list[at - 1])) != b)) {
+        s.place = at;
+        s.count_before = own[i];
+      }
+    }
+    __syncthreads();
+    const uint32_t first = s.place;
+    const uint64_t start = s.count_before;
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i)
+      if (bin[i] == b) f(2 * threadIdx.x + i, first, own[i] - start, mass[i]);
+    __syncthreads();
+  };
+  uint64_t all = ends.total, count = whole.there;
+  if (ends.end < BINS) {
+    if (ends.p == ends.end) {
+      in_bin(ends.end, [&](uint32_t at, uint32_t first, uint64_t start, uint64_t size) {
+        start += ends.end_before;
+        if (start <= ends.need - 1 && ends.need - 1 < start + size) {
+          s.mass_before = start + size;
+          s.found = at - first + 1;
+        }
+      });
+      all = s.mass_before;
+      count = larger + s.found;
+    }
+    if (ends.m == ends.end) {
+      uint64_t n_least, mass_least;
+      block_scan<THREADS>(many, s.wave, &n_least);
+      block_scan<THREADS>(weighs, s.wave, &mass_least);
+      if (larger + n_least < count) {
+        count = larger + n_least;
+        all = ends.end_before + mass_least;
+      }
+    }
+  }
+  const uint64_t unit = Row::drawn(u, all);
+  uint64_t at_bin;
+  const uint32_t b = ends.bin_of(s, unit, &at_bin);
+  in_bin(b, [&](uint32_t at, uint32_t, uint64_t start, uint64_t size) {
+    start += at_bin;
+    if (start <= unit && unit < start + size) s.chunk = at;
+  });
+  const uint64_t e = list[s.chunk];
+  *d = Result{(uint32_t)e, (uint32_t)count, row.log_share(listed_score(e), all)};
+  return true;
+}
+// The draw from the lists of a row's parts; false: one of them is none.  The j-th entries of all parts, j = k / parts rounded up, have
+// k entries up to the last of them: what comes after that one is not among the k best.
+__device__ __forceinline__ bool draw_joined(ListShared<THREADS>& s, const RowSpace& w, uint32_t parts, const Settings& o, double u, Result* d) {
+  constexpr int BT = THREADS;
+  const uint32_t lane = threadIdx.x & 63, k = o.greedy() ? 1 : o.top_k, j = (k + parts - 1) / parts;
+  const uint32_t count = lane < parts ? w.part_count[lane] : 0;
+  uint64_t last = lane >= parts ? 0 : count >= j && count != MANY_EQUAL ? w.part_list[lane][j - 1] : LIST_END;
+  if (threadIdx.x == 0) s.n = 0;
+  if (__ballot(count == MANY_EQUAL)) return false;  // every wavefront sees the same counts
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) last = max(last, shfl_xor_u64(last, m));
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < parts * PART_K; i += BT) {
+    const uint32_t n = (uint32_t)__shfl((int)count, (int)(i / PART_K), 64);
+    if (i % PART_K < n) {
+      const uint64_t e = w.part_list[i / PART_K][i % PART_K];
+      if (e <= last) s.list[atomicAdd(&s.n, 1u)] = e;
+    }
+  }
+  static_assert(MAX_PARTS * PART_K <= CAP<BT> && PART_K % 64 == 0, "all lists at once, a wavefront in one of them");
+  __syncthreads();
+  const uint32_t m = s.n;
+  *d = !m ? nothing_to_draw() : o.greedy() ? first_listed(s, m) : draw_list(s, m, o, u);
+  return true;
+}
+
 // A workgroup of 1024 threads has a row; `left`: only the rows that draw_short_kernel has left.
 template <typename T>
-__global__ __launch_bounds__(THREADS) void draw_kernel(DrawArgs a, bool left) {
+__global__ __launch_bounds__(THREADS) void draw_kernel(DrawArgs a, bool left, Parts p) {
   __shared__ Shared<THREADS> s;
   const uint32_t r = blockIdx.x;
   if (left && a.tokens[r * a.tokens_stride] != NOT_DRAWN) return;
   const Settings o(a, r);
-  const Result d = draw_row<T, THREADS>((const T*)a.logits + r * a.stride, a.columns, s, o, uniform_of(a, r));
+  const double u = uniform_of(a, r);
+  Result d;
+  bool done = false;
+  if constexpr (sizeof(T) == 4)
+    if (p.parts) {
+      const RowSpace& w = p.space[r];
+      done = o.few(PART_K, false) ? draw_joined(s.large.some.l, w, p.parts, o, u, &d) : draw_collected(s, w, p.parts, a.columns, o, u, &d);
+    }
+  if (!done) {
+    __syncthreads();
+    d = draw_row<T, THREADS>((const T*)a.logits + r * a.stride, a.columns, s, o, u);
+  }
   if (threadIdx.x == 0) store_result(a, r, d);
 }
 
@@ -1291,21 +1693,39 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void draw_short_kernel(DrawArgs a
 
 // Which workgroups draw.  One of 256 threads for a row that is short, and for any where there are more rows than CUs: four of them share a
 // CU.  16-bit logits are the exception: a long row of which many entries can stay is drawn from by value, which takes a CU.  (us, 1024 /
-// 256 threads: 2,000 x 8,000 bf16 by top-p 166 / 74, top-k of 50 95 / 23; 1,000 x 20,000 by top-p 105 / 72, 400 x 30,000 48 / 61,
-// 256 x 131,072 45 / 241, 1,000 x 60,000 top-k of 50 56 / 30; fp32 100 x 20,000 by top-p 46 / 39, 600 x 100,000 337 / 248,
-// 40 x 100,003 19 / 43.)
+// 256 threads: 2,000 x 8,000 bf16 by top-p 146 / 76, top-k of 50 80 / 23; 1,000 x 20,000 by top-p 82 / 74, 400 x 30,000 42 / 63,
+// 256 x 131,072 37 / 253; 400 x 100,000 top-k of 50 33 / 25; fp32 100 x 20,000 by top-p 46 / 39, 600 x 100,000 322 / 244,
+// 40 x 100,003 top-k of 40 18 / 23.)
 constexpr uint32_t SHORT_ROW_16 = 20480, SHORT_ROW_32 = 32768, MANY_ROWS = 256;
+// Parts of a row: two workgroups a CU, of at least 4,096 columns each.  Four and more are worth the launches.
+Parts parts_of(size_t size, uint32_t rows, uint32_t columns, void* workspace) {
+  Parts p{};
+  if (size != 4 || !rows || columns <= SHORT_ROW_32) return p;
+  const uint32_t parts = std::min(std::min(2 * 256 / rows, columns / 4096), MAX_PARTS);
+  if (parts < 4) return p;
+  p.span = ((columns + parts - 1) / parts + 63) / 64 * 64;
+  p.parts = (columns + p.span - 1) / p.span;
+  p.space = (RowSpace*)workspace;
+  return p;
+}
+
 template <typename T>
-void launch_draw(const DrawArgs& a, hipStream_t st) {
+void launch_draw(const DrawArgs& a, const Parts& p, hipStream_t st) {
   const dim3 grid(a.rows), few(SHORT_THREADS), all(THREADS);
   const bool many = a.rows > MANY_ROWS;
   if (a.columns <= (sizeof(T) == 4 ? SHORT_ROW_32 : SHORT_ROW_16) || (many && sizeof(T) == 4)) {
     hipLaunchKernelGGL(draw_short_kernel<T>, grid, few, 0, st, a, false);
   } else if (many) {
     hipLaunchKernelGGL(draw_short_kernel<T>, grid, few, 0, st, a, true);
-    hipLaunchKernelGGL(draw_kernel<T>, grid, all, 0, st, a, true);
+    hipLaunchKernelGGL(draw_kernel<T>, grid, all, 0, st, a, true, Parts{});
   } else {
-    hipLaunchKernelGGL(draw_kernel<T>, grid, all, 0, st, a, false);
+    if (p.parts) {
+      const dim3 parts(a.rows * p.parts);
+      hipLaunchKernelGGL(parts_kernel, parts, few, 0, st, a, p);
+      hipLaunchKernelGGL(fill_kernel, parts, few, 0, st, a, p);
+      hipLaunchKernelGGL(collect_kernel, parts, few, 0, st, a, p);
+    }
+    hipLaunchKernelGGL(draw_kernel<T>, grid, all, 0, st, a, false, p);
   }
 }
 
@@ -1318,7 +1738,7 @@ extern "C" int sky_logits_draw_workspace(int dtype, uint32_t rows, uint32_t colu
   uint64_t stride = 0;
   if (!bytes) return fail(SKY_ERR_ARG, "sky_logits_draw_workspace: null output");
   SKY_TRY(check_rows("sky_logits_draw_workspace", "logits", bytes, dtype, rows, columns, &stride));
-  *bytes = 0;
+  *bytes = parts_of(dtype_size(dtype), rows, columns, nullptr).parts ? rows * sizeof(RowSpace) : 0;
   return SKY_OK;
 }
 
@@ -1351,12 +1771,13 @@ extern "C" int sky_logits_draw(const void* logits, int dtype, uint32_t rows, uin
     const DrawArgs a{(const char*)logits + r * row_stride * dtype_size(dtype), row_stride, columns, std::min(SLICE, rows - r), from(d.temperature),
                      from(d.top_k), from(d.top_p), from(d.min_p), from(uniforms), philox_seed, first_walker + r, step,
                      tokens + r * tokens_stride, tokens_stride, from(logprobs), from(kept)};
+    const Parts p = workspace ? parts_of(dtype_size(dtype), rows, columns, workspace) : Parts{};
     if (dtype == SKY_F32)
-      launch_draw<float>(a, st);
+      launch_draw<float>(a, p, st);
     else if (dtype == SKY_F16)
-      launch_draw<_Float16>(a, st);
+      launch_draw<_Float16>(a, p, st);
     else
-      launch_draw<__bf16>(a, st);
+      launch_draw<__bf16>(a, p, st);
     SKY_TRY(check_launch());
   }
   return SKY_OK;

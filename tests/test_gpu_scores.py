@@ -319,6 +319,26 @@ def test_draw_of_many_long_rows(capi, orc, dtype, columns):
              top_p=rng.choice([1.0, 0.9, 0.5], n), min_p=rng.choice([0.0, 0.0, 0.02], n), u=rng.random(n))
 
 
+@pytest.mark.parametrize("rows,columns", [(1, 131072), (61, 40011), (128, 33000)])
+def test_draw_of_a_few_long_rows_with_a_workspace(capi, orc, rows, columns):
+    assert capi.logits_draw_workspace(capi.F32, rows, columns) > 0 and capi.logits_draw_workspace(capi.F32, 129, columns) == 0
+    assert capi.logits_draw_workspace(capi.BF16, rows, columns) == 0 and capi.logits_draw_workspace(capi.F32, rows, 32768) == 0
+    rng = np.random.default_rng(columns)
+    for n in range(3):
+        x = rng.normal(0, 3, (rows, columns)).astype(np.float32)
+        x[3::8] = rng.integers(-9, 10, x[3::8].shape)  # bins of one value, more than a list holds
+        x[4::8] = np.where(rng.random(x[4::8].shape) < 0.97, -INF, x[4::8])
+        x[5::8] = np.round(x[5::8] * 64) / 64
+        x[6::8, : columns // 2] = -INF
+        x[7::16] *= np.float32(1e-6)
+        if rows > 9:
+            x[9] = -INF
+        k = rng.choice([0, 0, 0, 1, 50, 128, 129, 3000], rows)
+        run_draw(capi, orc, x, "f32", pad=n, lead=n, t=rng.choice([0.0, 0.3, 1.0, 2.0, 50.0], rows, p=[0.1, 0.2, 0.4, 0.2, 0.1]), top_k=k if n else 0 * k,
+                 top_p=rng.choice([1.0, 0.97, 0.6, 1e-6, 0.0], rows), min_p=rng.choice([0.0, 0.0, 0.02, 0.5, 1e-12], rows),
+                 u=rng.choice([0.0, 1 - 2.0 ** -53], rows) if n == 2 else rng.random(rows), workspace=True)
+
+
 def test_draw_of_more_rows_than_a_launch_has(capi):
     rows = (1 << 21) + 5
     x = np.random.default_rng(13).normal(0, 2, (rows, 2)).astype(np.float16)
