@@ -1243,7 +1243,12 @@ struct RowSpace {  // of a row in the workspace
   uint64_t part_list[MAX_PARTS][PART_K];
   uint32_t count[BINS];
   uint32_t most[MAX_PARTS], least[MAX_PARTS], there[MAX_PARTS], part_count[MAX_PARTS];
-  uint32_t n, unused[3];                    // entries of `list`
+  // by collect_kernel: the bins in which top-p, min-p or the first of them end the row, what lies before the latter's, how many entries
+  // do, and the mass of all; the bins [first, last] in which the drawn unit may lie, and what lies before each
+  uint64_t end_before, total, start[64];
+  uint32_t p, m, end, larger, first, last;
+  float z_least;
+  uint32_t n;  // entries of `list`, more than it holds where they or the bins are too many
 };
 struct Parts {
   RowSpace* space;
@@ -1281,65 +1286,6 @@ __device__ __forceinline__ float least_of_min_p(const Row& row, float min_p, uin
   }
   return P::value(min(lo + 1, most));
 }
-// Where the row ends and where the drawn unit may lie, from the bins, BINS / BT a thread: by every thread.
-template <int BT>
-struct Ends {
-  static constexpr uint32_t PER = BINS / BT;
-  uint64_t mine[PER], before, total;  // the thread's bins, and what lies before them
-  uint32_t p, m, end;                 // bins in which top-p and min-p end, the first of them; BINS: none
-  uint64_t need, end_before, end_mass;
-  template <typename F>
-  __device__ __forceinline__ void each_own(F f) const {
-    uint64_t b = before;
-#pragma unroll
-    for (uint32_t i = 0; i < PER; ++i) {
-      f(PER * threadIdx.x + i, b, mine[i]);
-      b += mine[i];
-    }
-  }
-  // the bin that holds a unit of mass; `at`: what lies before it
-  __device__ __forceinline__ uint32_t bin_of(Shared<BT>& s, uint64_t unit, uint64_t* at) const {
-    __syncthreads();
-    each_own([&](uint32_t b, uint64_t start, uint64_t size) {
-      if (start <= unit && unit < start + size) {
-        s.found = b;
-        s.mass_before = start;
-      }
-    });
-    __syncthreads();
-    *at = s.mass_before;
-    return s.found;
-  }
-  __device__ __forceinline__ Ends(Shared<BT>& s, const RowSpace& w, const Settings& o, const Bins& bins, float z_least) {
-    uint64_t sum = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < PER; ++i) sum += mine[i] = w.bin[PER * threadIdx.x + i];
-    before = block_scan<BT>(sum, s.wave, &total);
-    p = m = BINS;
-    need = 0;
-    if (o.top_p < 1.0f) {
-      need = Row::needed(o.top_p, total);
-      p = bin_of(s, need - 1, &end_before);
-    }
-    if (o.min_p > 0.0f && bins.has(z_least)) m = bins.of(z_least);
-    end = min(p, m);
-    end_before = 0;
-    end_mass = total;
-    if (end < BINS) {
-      __syncthreads();
-      each_own([&](uint32_t b, uint64_t start, uint64_t size) {
-        if (b == end) {
-          s.mass_before = start;
-          s.count_before = size;
-        }
-      });
-      __syncthreads();
-      end_before = s.mass_before;
-      end_mass = s.count_before;
-    }
-  }
-};
-
 __global__ __launch_bounds__(SHORT_THREADS, 4) void parts_kernel(DrawArgs a, Parts p) {
   constexpr int BT = SHORT_THREADS;
   using T = float;
@@ -1422,22 +1368,30 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void parts_kernel(DrawArgs a, Par
   if (tid < m) w.part_list[part][tid] = l.list[tid];
 }
 
-// f(value, column) for the entries of a part from `low` on.
+// f(four values, their first column, bits of those from `low` on) for the pieces of a part, and for the odd entries one by one; values
+// that are not meant are `low`.
 template <typename F>
 __device__ __forceinline__ void each_of_part(const Reader<float, SHORT_THREADS>& in, float low, F f) {
   using P = Places<float>;
-  auto one = [&](uint32_t bits, uint32_t c) {
-    const uint32_t q = place_of_bits<float>(bits);
-    const float z = P::value(q);
-    if (q && z >= low) f(z, c);
-  };
   in.stream([&](uint4 v, uint32_t c) {
-    one(v.x, c);
-    one(v.y, c + 1);
-    one(v.z, c + 2);
-    one(v.w, c + 3);
+    const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+    float z[4];
+    uint32_t wanted = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t q = place_of_bits<float>(word[i]);
+      const bool mine = q && P::value(q) >= low;
+      z[i] = mine ? P::value(q) : low;
+      wanted |= mine ? 1u << i : 0u;
+    }
+    f(z, c, wanted);
   });
-  if (in.whole + threadIdx.x < in.columns) one(__float_as_uint(in.x[in.whole + threadIdx.x]), in.whole + threadIdx.x);
+  const uint32_t c = in.whole + threadIdx.x;
+  if (c < in.columns) {
+    const uint32_t q = place_of_bits<float>(__float_as_uint(in.x[c]));
+    const float z[4] = {q ? P::value(q) : low, low, low, low};
+    f(z, c, q && z[0] >= low ? 1u : 0u);
+  }
 }
 
 __global__ __launch_bounds__(SHORT_THREADS, 4) void fill_kernel(DrawArgs a, Parts p) {
@@ -1457,10 +1411,17 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void fill_kernel(DrawArgs a, Part
   }
   __syncthreads();
   const Reader<float, SHORT_THREADS> in((const float*)a.logits + r * a.stride + start, min(p.span, a.columns - start));
-  each_of_part(in, bins.low, [&](float z, uint32_t) {
-    const uint32_t b = bins.of(z);
-    atomicAdd((unsigned long long*)&bin[b], (unsigned long long)row.units(z));
-    atomicAdd(&count[b], 1u);
+  each_of_part(in, bins.low, [&](const float (&z)[4], uint32_t, uint32_t wanted) {
+    uint64_t units[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) units[i] = row.units(z[i]);  // without branches: beside one another
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (wanted >> i & 1) {
+        const uint32_t b = bins.of(z[i]);
+        atomicAdd((unsigned long long*)&bin[b], (unsigned long long)units[i]);
+        atomicAdd(&count[b], 1u);
+      }
   });
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < BINS; i += SHORT_THREADS)
@@ -1471,114 +1432,187 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void fill_kernel(DrawArgs a, Part
 }
 
 __global__ __launch_bounds__(SHORT_THREADS, 4) void collect_kernel(DrawArgs a, Parts p) {
-  __shared__ Shared<SHORT_THREADS> s;
-  const uint32_t r = blockIdx.x / p.parts, start = blockIdx.x % p.parts * p.span;
+  constexpr int BT = SHORT_THREADS;
+  constexpr uint32_t PER = BINS / BT;
+  __shared__ Shared<BT> s;
+  ListShared<BT>& l = s.large.some.l;
+  const uint32_t r = blockIdx.x / p.parts, part = blockIdx.x % p.parts, start = part * p.span, tid = threadIdx.x;
   RowSpace& w = p.space[r];
   const Settings o(a, r);
   if (o.few(PART_K, false)) return;
+  // what does not depend on one another is asked for at once: the kernel is a chain of waits
+  uint64_t mine[PER], sum = 0, total;  // the thread's bins
+  uint32_t counts[PER];
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) mine[i] = w.bin[PER * tid + i];
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) counts[i] = w.count[PER * tid + i];
+  const double u = uniform_of(a, r);
   const Whole whole(w, p.parts);
   if (!drawn_in_parts(o, whole)) return;
   const Row row(o.temperature, key_score(whole.most), fraction_bits(a.columns));
   const Bins bins = bins_of(row, whole);
   const float z_least = o.min_p > 0.0f ? least_of_min_p(row, o.min_p, whole.most) : 0.0f;
-  const Ends<SHORT_THREADS> ends(s, w, o, bins, z_least);
-  const double u = uniform_of(a, r);
-  uint64_t before;
-  const uint64_t least_mass = ends.end < BINS ? max(ends.end_before, (uint64_t)1) : ends.total;
-  const uint32_t first = ends.bin_of(s, Row::drawn(u, least_mass), &before);
-  const uint32_t last = ends.bin_of(s, Row::drawn(u, ends.end_before + ends.end_mass), &before);
-  const Reader<float, SHORT_THREADS> in((const float*)a.logits + r * a.stride + start, min(p.span, a.columns - start));
-  each_of_part(in, bins.low, [&](float z, uint32_t c) {
-    const uint32_t b = bins.of(z);
-    if (b == ends.end || (b >= first && b <= last)) {
-      const uint32_t at = atomicAdd(&w.n, 1u);
-      if (at < CAP<THREADS>) w.list[at] = listed(z, start + c);
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) sum += mine[i];
+  if (tid == 0) l.n = 0;
+  const uint64_t before = block_scan<BT>(sum, s.wave, &total);
+  auto each_own = [&](auto f) {
+    uint64_t at = before;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) {
+      f(PER * tid + i, at, mine[i]);
+      at += mine[i];
     }
+  };
+  auto bin_of = [&](uint64_t unit) {  // the bin that holds a unit of mass
+    __syncthreads();
+    each_own([&](uint32_t b, uint64_t at, uint64_t size) {
+      if (at <= unit && unit < at + size) s.found = b;
+    });
+    __syncthreads();
+    return s.found;
+  };
+  const uint32_t by_p = o.top_p < 1.0f ? bin_of(Row::needed(o.top_p, total) - 1) : BINS;
+  const uint32_t by_m = o.min_p > 0.0f && bins.has(z_least) ? bins.of(z_least) : BINS, end = min(by_p, by_m);
+  uint64_t least = total, most = total, end_before = 0;  // of what stays
+  if (end < BINS) {
+    __syncthreads();
+    each_own([&](uint32_t b, uint64_t at, uint64_t size) {
+      if (b == end) {
+        s.mass_before = at;
+        s.count_before = size;
+      }
+    });
+    __syncthreads();
+    end_before = s.mass_before;
+    least = max(end_before, (uint64_t)1);
+    most = end_before + s.count_before;
+  }
+  const uint32_t first = bin_of(Row::drawn(u, least)), last = bin_of(Row::drawn(u, most));
+  constexpr uint32_t STARTS = sizeof(w.start) / sizeof(w.start[0]);
+  if (part == 0) {
+    each_own([&](uint32_t b, uint64_t at, uint64_t) {
+      if (b >= first && b <= last && b - first < STARTS) w.start[b - first] = at;
+    });
+    uint64_t many = 0, larger;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) many += PER * tid + i < end ? counts[i] : 0;
+    block_scan<BT>(many, s.wave, &larger);
+    if (tid == 0) {
+      w.end_before = end_before;
+      w.total = total;
+      w.p = by_p;
+      w.m = by_m;
+      w.end = end;
+      w.larger = (uint32_t)larger;
+      w.first = first;
+      w.last = last;
+      w.z_least = z_least;
+      if (last - first >= STARTS) atomicAdd(&w.n, CAP<THREADS> + 1);
+    }
+  }
+  const Reader<float, BT> in((const float*)a.logits + r * a.stride + start, min(p.span, a.columns - start));
+  each_of_part(in, bins.low, [&](const float (&z)[4], uint32_t c, uint32_t wanted) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = bins.of(z[i]);
+      found |= b == end || (b >= first && b <= last) ? 1u << i : 0u;
+    }
+    found &= wanted;
+    if (found)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (found >> i & 1) {
+          const uint32_t at = atomicAdd(&l.n, 1u);
+          if (at < CAP<BT>) l.list[at] = listed(z[i], start + c + i);
+        }
   });
+  __syncthreads();
+  const uint32_t n = l.n;
+  if (tid == 0 && n) s.place = atomicAdd(&w.n, n > CAP<BT> ? CAP<THREADS> + 1 : n);
+  __syncthreads();
+  const uint32_t at = s.place;
+  for (uint32_t i = tid; i < min(n, CAP<BT>); i += BT)
+    if (at + i < CAP<THREADS>) w.list[at + i] = l.list[i];
 }
 
 // The draw from what the parts have left; false: it is none of theirs.
 __device__ __forceinline__ bool draw_collected(Shared<THREADS>& s, const RowSpace& w, uint32_t parts, uint32_t columns, const Settings& o, double u, Result* d) {
-  constexpr uint32_t PER = BINS / THREADS;
-  static_assert(PER == 2 && CAP<THREADS> == 2 * THREADS, "two bins and two entries a thread");
+  static_assert(CAP<THREADS> == 2 * THREADS, "two entries a thread");
+  const uint32_t lane = threadIdx.x & 63, n = w.n, end = w.end, by_p = w.p, by_m = w.m, first = w.first, last = w.last, larger = w.larger;
+  const uint64_t total = w.total, end_before = w.end_before, starts = w.start[lane], start = lane <= last - first ? starts : ~0ull;
+  const uint64_t listed0 = w.list[threadIdx.x], listed1 = w.list[THREADS + threadIdx.x];  // whatever they are beyond n
+  const float z_least = w.z_least;
   const Whole whole(w, parts);
-  const uint32_t n = w.n;
   if (!drawn_in_parts(o, whole) || n > CAP<THREADS>) return false;
   const Row row(o.temperature, key_score(whole.most), fraction_bits(columns));
   const Bins bins = bins_of(row, whole);
   uint64_t* const list = s.large.some.l.list;
-  for (uint32_t i = threadIdx.x; i < n; i += THREADS) list[i] = w.list[i];
-  const float z_least = o.min_p > 0.0f ? least_of_min_p(row, o.min_p, whole.most) : 0.0f;
-  const Ends<THREADS> ends(s, w, o, bins, z_least);
-  // entries in the bins before the one that ends the row
-  uint64_t mine = 0, larger;
-#pragma unroll
-  for (uint32_t i = 0; i < PER; ++i) mine += PER * threadIdx.x + i < ends.end ? w.count[PER * threadIdx.x + i] : 0;
-  block_scan<THREADS>(mine, s.wave, &larger);  // its barriers publish the list
+  list[threadIdx.x] = listed0;
+  list[THREADS + threadIdx.x] = listed1;
+  __syncthreads();
   sort_list<THREADS>(list, n);
   uint32_t bin[2], many = 0;
   uint64_t mass[2], weighs = 0, sum;
-  float z[2];
+  bool begins[2];  // a bin's entries
 #pragma unroll
   for (uint32_t i = 0; i < 2; ++i) {
     const uint32_t at = 2 * threadIdx.x + i;
-    z[i] = at < n ? listed_score(list[at]) : 0.0f;
-    bin[i] = at < n ? bins.of(z[i]) : BINS + 1;
-    mass[i] = at < n ? row.units(z[i]) : 0;
-    if (bin[i] == ends.m && z[i] >= z_least) {
+    const float z = at < n ? listed_score(list[at]) : row.zmax;
+    bin[i] = at < n ? bins.of(z) : BINS + 1;
+    begins[i] = at < n && (at == 0 || bins.of(listed_score(list[at - 1])) != bin[i]);
+    mass[i] = row.units(z);
+    if (at >= n) mass[i] = 0;
+    if (bin[i] == by_m && z >= z_least) {
       ++many;
       weighs += mass[i];
     }
   }
   const uint64_t before = block_scan<THREADS>(mass[0] + mass[1], s.wave, &sum), own[2] = {before, before + mass[0]};
-  // f(entry, what lies before it in its bin) for the entries of bin b
-  auto in_bin = [&](uint32_t b, auto f) {
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-      const uint32_t at = 2 * threadIdx.x + i;
-      if (bin[i] == b && (at == 0 || bins.of(listed_score(list[at - 1])) != b)) {
-        s.place = at;
-        s.count_before = own[i];
-      }
-    }
-    __syncthreads();
-    const uint32_t first = s.place;
-    const uint64_t start = s.count_before;
+  // f(entry, the bin's first, what lies before the entry, its mass) for the entries of bin b, before which `at` lies
+  auto in_bin = [&](uint32_t b, uint64_t at, auto f) {
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i)
-      if (bin[i] == b) f(2 * threadIdx.x + i, first, own[i] - start, mass[i]);
+      if (bin[i] == b && begins[i]) {
+        s.place = 2 * threadIdx.x + i;
+        s.count_before = own[i];
+      }
+    __syncthreads();
+    const uint32_t from = s.place;
+    at -= s.count_before;
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i)
+      if (bin[i] == b) f(2 * threadIdx.x + i, from, at + own[i], mass[i]);
     __syncthreads();
   };
-  uint64_t all = ends.total, count = whole.there;
-  if (ends.end < BINS) {
-    if (ends.p == ends.end) {
-      in_bin(ends.end, [&](uint32_t at, uint32_t first, uint64_t start, uint64_t size) {
-        start += ends.end_before;
-        if (start <= ends.need - 1 && ends.need - 1 < start + size) {
-          s.mass_before = start + size;
-          s.found = at - first + 1;
-        }
-      });
-      all = s.mass_before;
-      count = larger + s.found;
-    }
-    if (ends.m == ends.end) {
-      uint64_t n_least, mass_least;
-      block_scan<THREADS>(many, s.wave, &n_least);
-      block_scan<THREADS>(weighs, s.wave, &mass_least);
-      if (larger + n_least < count) {
-        count = larger + n_least;
-        all = ends.end_before + mass_least;
+  uint64_t all = total, count = whole.there;
+  if (by_p == end && end < BINS) {
+    const uint64_t unit = Row::needed(o.top_p, total) - 1;
+    in_bin(end, end_before, [&](uint32_t at, uint32_t from, uint64_t b, uint64_t size) {
+      if (b <= unit && unit < b + size) {
+        s.mass_before = b + size;
+        s.found = at - from + 1;
       }
+    });
+    all = s.mass_before;
+    count = larger + s.found;
+  }
+  if (by_m == end && end < BINS) {
+    uint64_t n_least, mass_least;
+    block_scan<THREADS>(many, s.wave, &n_least);
+    block_scan<THREADS>(weighs, s.wave, &mass_least);
+    if (larger + n_least < count) {
+      count = larger + n_least;
+      all = end_before + mass_least;
     }
   }
+  // of the bins that may hold it the last that begins before the drawn unit or with it does
   const uint64_t unit = Row::drawn(u, all);
-  uint64_t at_bin;
-  const uint32_t b = ends.bin_of(s, unit, &at_bin);
-  in_bin(b, [&](uint32_t at, uint32_t, uint64_t start, uint64_t size) {
-    start += at_bin;
-    if (start <= unit && unit < start + size) s.chunk = at;
+  const int which = 63 - (int)__builtin_clzll(__ballot(start <= unit));
+  in_bin(first + (uint32_t)which, shfl_u64(start, which), [&](uint32_t at, uint32_t, uint64_t b, uint64_t size) {
+    if (b <= unit && unit < b + size) s.chunk = at;
   });
   const uint64_t e = list[s.chunk];
   *d = Result{(uint32_t)e, (uint32_t)count, row.log_share(listed_score(e), all)};
@@ -1610,8 +1644,9 @@ __device__ __forceinline__ bool draw_joined(ListShared<THREADS>& s, const RowSpa
   return true;
 }
 
-// A workgroup of 1024 threads has a row; `left`: only the rows that draw_short_kernel has left.
-template <typename T>
+// A workgroup of 1024 threads has a row; `left`: only the rows that draw_short_kernel has left.  PARTS: rows that their parts have been
+// at (a kernel of its own: the others do without its registers).
+template <typename T, bool PARTS>
 __global__ __launch_bounds__(THREADS) void draw_kernel(DrawArgs a, bool left, Parts p) {
   __shared__ Shared<THREADS> s;
   const uint32_t r = blockIdx.x;
@@ -1620,15 +1655,12 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(DrawArgs a, bool left, Pa
   const double u = uniform_of(a, r);
   Result d;
   bool done = false;
-  if constexpr (sizeof(T) == 4)
-    if (p.parts) {
-      const RowSpace& w = p.space[r];
-      done = o.few(PART_K, false) ? draw_joined(s.large.some.l, w, p.parts, o, u, &d) : draw_collected(s, w, p.parts, a.columns, o, u, &d);
-    }
-  if (!done) {
+  if constexpr (PARTS) {
+    const RowSpace& w = p.space[r];
+    done = o.few(PART_K, false) ? draw_joined(s.large.some.l, w, p.parts, o, u, &d) : draw_collected(s, w, p.parts, a.columns, o, u, &d);
     __syncthreads();
-    d = draw_row<T, THREADS>((const T*)a.logits + r * a.stride, a.columns, s, o, u);
   }
+  if (!done) d = draw_row<T, THREADS>((const T*)a.logits + r * a.stride, a.columns, s, o, u);
   if (threadIdx.x == 0) store_result(a, r, d);
 }
 
@@ -1697,12 +1729,15 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void draw_short_kernel(DrawArgs a
 // 256 x 131,072 37 / 253; 400 x 100,000 top-k of 50 33 / 25; fp32 100 x 20,000 by top-p 46 / 39, 600 x 100,000 322 / 244,
 // 40 x 100,003 top-k of 40 18 / 23.)
 constexpr uint32_t SHORT_ROW_16 = 20480, SHORT_ROW_32 = 32768, MANY_ROWS = 256;
-// Parts of a row: two workgroups a CU, of at least 4,096 columns each.  Four and more are worth the launches.
+// Parts of a row: two workgroups a CU, of at least 4,096 columns each, eight and more.  What rows of few candidates lose is the launches of
+// kernels that have nothing to do with them.  (us, a workgroup a row / in parts, fp32: 8 x 131,072 by top-p 114 / 48, top-k of 50
+// 19 / 21; 40 x 100,003 by top-p 95 / 49, top-k of 40 19 / 22; 128 x 100,003, by four, 107 / 95 and 27 / 31.  16-bit rows, whose values are
+// counted: 65,536 by top-k of 50 11 / 17.)
 Parts parts_of(size_t size, uint32_t rows, uint32_t columns, void* workspace) {
   Parts p{};
   if (size != 4 || !rows || columns <= SHORT_ROW_32) return p;
   const uint32_t parts = std::min(std::min(2 * 256 / rows, columns / 4096), MAX_PARTS);
-  if (parts < 4) return p;
+  if (parts < 8) return p;
   p.span = ((columns + parts - 1) / parts + 63) / 64 * 64;
   p.parts = (columns + p.span - 1) / p.span;
   p.space = (RowSpace*)workspace;
@@ -1717,15 +1752,18 @@ void launch_draw(const DrawArgs& a, const Parts& p, hipStream_t st) {
     hipLaunchKernelGGL(draw_short_kernel<T>, grid, few, 0, st, a, false);
   } else if (many) {
     hipLaunchKernelGGL(draw_short_kernel<T>, grid, few, 0, st, a, true);
-    hipLaunchKernelGGL(draw_kernel<T>, grid, all, 0, st, a, true, Parts{});
+    hipLaunchKernelGGL((draw_kernel<T, false>), grid, all, 0, st, a, true, p);
   } else {
-    if (p.parts) {
-      const dim3 parts(a.rows * p.parts);
-      hipLaunchKernelGGL(parts_kernel, parts, few, 0, st, a, p);
-      hipLaunchKernelGGL(fill_kernel, parts, few, 0, st, a, p);
-      hipLaunchKernelGGL(collect_kernel, parts, few, 0, st, a, p);
-    }
-    hipLaunchKernelGGL(draw_kernel<T>, grid, all, 0, st, a, false, p);
+    if constexpr (sizeof(T) == 4)
+      if (p.parts) {
+        const dim3 parts(a.rows * p.parts);
+        hipLaunchKernelGGL(parts_kernel, parts, few, 0, st, a, p);
+        hipLaunchKernelGGL(fill_kernel, parts, few, 0, st, a, p);
+        hipLaunchKernelGGL(collect_kernel, parts, few, 0, st, a, p);
+        hipLaunchKernelGGL((draw_kernel<T, true>), grid, all, 0, st, a, false, p);
+        return;
+      }
+    hipLaunchKernelGGL((draw_kernel<T, false>), grid, all, 0, st, a, false, p);
   }
 }
 
