@@ -2,16 +2,20 @@
 // weigh w = exp((z - zmax) / T); what stays of the row is always a beginning of that order (top-k, top-p and min-p each
 // cut off an end), and the drawn entry is the first whose weights, summed in the order, pass u times what stays weighs.  So
 // everything is one question, asked up to three times: which entry of the order holds rank k, or the unit of mass t?  A row is read
-// once to answer it, and in places a second time; it is never sorted.  What is done depends on how many entries can matter:
+// once to answer it, and in places again; it is never sorted.  What is done depends on how many entries can matter:
 //
 //   list    at most CAP entries can stay: they are listed in LDS and sorted.  Rows of which a grammar leaves a few, top-k of up to
 //           SMALL_K (the k-th largest of the threads' largest entries is no larger than the k-th largest entry) and min-p without top-p.
+//           Bound by the reading: 4,096 x 65,536 f16 with a few neighbours each 113 us, 4.7 TB/s.
 //   values  16-bit logits have at most 65,536 values: they are counted by value, in 16-bit counters that take 128 KB of
-//           LDS, and the rest (weights, prefixes, borders) is a matter of the values that occur, a few thousand.
+//           LDS, and the rest (weights, prefixes, borders) is a matter of the values that occur, a few thousand.  Bound by the LDS atomics
+//           and the second reading, for the columns of equal entries: 256 x 131,072 bf16 by top-p 37 us, 1.8 TB/s.
 //   bins    the others (fp32, shorter rows, rows in which a counter runs over): weights are summed in BINS bins of equal width between the largest
 //           value and the smallest that weighs anything; the bin that holds the answer is listed and sorted, and
 //           when it does not fit the list it becomes the next interval.  That then lies between the smallest and largest value met in it, so
-//           that two different values never stay together, and a bin of one value is a matter of counting.
+//           that two different values never stay together, and a bin of one value is a matter of counting.  Bound by the fp64 weights
+//           and three readings by one CU: 600 x 100,000 fp32 by top-p 244 us.
+//   parts   the bins of a few long fp32 rows by several workgroups a row: 40 x 100,003 by top-p 49 us instead of 95.
 //
 // Weights are summed in whole numbers (2^-S of the largest weight, S = 61 less the bits of the row's length, 50 at most): sums then do
 // not depend on the order of LDS atomics or of lanes.  They are rounded once each, by at most 2^-(S+1) of the largest weight; the

