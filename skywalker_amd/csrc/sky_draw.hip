@@ -1550,6 +1550,10 @@ __device__ __forceinline__ bool draw_collected(Shared<THREADS>& s, const RowSpac
   const uint64_t listed0 = w.list[threadIdx.x], listed1 = w.list[THREADS + threadIdx.x];  // whatever they are beyond n
   const float z_least = w.z_least;
   const Whole whole(w, parts);
+  if (!whole.there) {
+    *d = nothing_to_draw();
+    return true;
+  }
   if (!drawn_in_parts(o, whole) || n > CAP<THREADS>) return false;
   const Row row(o.temperature, key_score(whole.most), fraction_bits(columns));
   const Bins bins = bins_of(row, whole);
@@ -1752,21 +1756,24 @@ template <typename T>
 void launch_draw(const DrawArgs& a, const Parts& p, hipStream_t st) {
   const dim3 grid(a.rows), few(SHORT_THREADS), all(THREADS);
   const bool many = a.rows > MANY_ROWS;
-  if (a.columns <= (sizeof(T) == 4 ? SHORT_ROW_32 : SHORT_ROW_16) || (many && sizeof(T) == 4)) {
+  if constexpr (sizeof(T) == 4) {
+    if (many || a.columns <= SHORT_ROW_32) {
+      hipLaunchKernelGGL(draw_short_kernel<T>, grid, few, 0, st, a, false);
+    } else if (p.parts) {
+      const dim3 parts(a.rows * p.parts);
+      hipLaunchKernelGGL(parts_kernel, parts, few, 0, st, a, p);
+      hipLaunchKernelGGL(fill_kernel, parts, few, 0, st, a, p);
+      hipLaunchKernelGGL(collect_kernel, parts, few, 0, st, a, p);
+      hipLaunchKernelGGL((draw_kernel<T, true>), grid, all, 0, st, a, false, p);
+    } else {
+      hipLaunchKernelGGL((draw_kernel<T, false>), grid, all, 0, st, a, false, p);
+    }
+  } else if (a.columns <= SHORT_ROW_16) {
     hipLaunchKernelGGL(draw_short_kernel<T>, grid, few, 0, st, a, false);
   } else if (many) {
     hipLaunchKernelGGL(draw_short_kernel<T>, grid, few, 0, st, a, true);
     hipLaunchKernelGGL((draw_kernel<T, false>), grid, all, 0, st, a, true, p);
   } else {
-    if constexpr (sizeof(T) == 4)
-      if (p.parts) {
-        const dim3 parts(a.rows * p.parts);
-        hipLaunchKernelGGL(parts_kernel, parts, few, 0, st, a, p);
-        hipLaunchKernelGGL(fill_kernel, parts, few, 0, st, a, p);
-        hipLaunchKernelGGL(collect_kernel, parts, few, 0, st, a, p);
-        hipLaunchKernelGGL((draw_kernel<T, true>), grid, all, 0, st, a, false, p);
-        return;
-      }
     hipLaunchKernelGGL((draw_kernel<T, false>), grid, all, 0, st, a, false, p);
   }
 }
