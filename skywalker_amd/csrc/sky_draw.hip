@@ -1238,8 +1238,8 @@ __device__ __forceinline__ Result draw_row(const T* x, uint32_t columns, Shared<
 //   collect_kernel  the entries of the bin in which top-p or min-p ends the row, and of those bins in which the drawn unit lies for any end in that
 //                   bin (next to always one or two)
 //   draw_kernel     the draw from these
-// All sums are whole numbers in the same units, so that the ids are the same.  What does not fit (top-k above PART_K, min-p without top-p, rows with
-// next to nothing in them, lists that run over) is drawn from by draw_kernel alone.
+// All sums are whole numbers in the same units, so that the ids are the same.  What does not fit (top-k above PART_K, min-p without top-p, rows
+// with next to nothing in them, lists that run over) is drawn from by draw_kernel alone.
 constexpr uint32_t PART_K = SMALL_K<SHORT_THREADS>, MAX_PARTS = 16, MANY_EQUAL = 0xFFFFFFFFu;
 struct RowSpace {  // of a row in the workspace
   uint64_t bin[BINS];
@@ -1269,9 +1269,9 @@ struct Whole {
     there = (uint32_t)__shfl((int)group_scan_u32<64>(in ? w.there[lane] : 0), 63, 64);
   }
 };
-__device__ __forceinline__ bool drawn_in_parts(const Settings& o, const Whole& w) {
-  return w.there > CAP<THREADS> && !(o.top_k && o.top_k < w.there) && !(o.min_p > 0.0f && !(o.top_p < 1.0f));
-}
+// What its parts do with a row: list the best, sum up bins (of a row of more than CAP<THREADS> entries), or nothing.
+__device__ __forceinline__ bool listed_in_parts(const Settings& o) { return o.few(PART_K, false); }
+__device__ __forceinline__ bool summed_in_parts(const Settings& o) { return !o.greedy() && !o.top_k && !(o.min_p > 0.0f && !(o.top_p < 1.0f)); }
 __device__ __forceinline__ Bins bins_of(const Row& row, const Whole& w) {
   const float cut = (float)fmax((double)row.zmax - NO_MASS * row.t, -3.402823466e38);
   return Bins(row.zmax, fmaxf(key_score(w.least), cut));
@@ -1299,7 +1299,8 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void parts_kernel(DrawArgs a, Par
   const uint32_t r = blockIdx.x / p.parts, part = blockIdx.x % p.parts, start = part * p.span, tid = threadIdx.x;
   RowSpace& w = p.space[r];
   const Settings o(a, r);
-  const bool few = o.few(PART_K, false);
+  const bool few = listed_in_parts(o);
+  if (!few && !summed_in_parts(o)) return;
   Reader<T, BT> in((const T*)a.logits + r * a.stride + start, min(p.span, a.columns - start));
   if (!few) {  // what the next kernels add to
     for (uint32_t i = part * BT + tid; i < BINS; i += p.parts * BT) {
@@ -1404,9 +1405,9 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void fill_kernel(DrawArgs a, Part
   const uint32_t r = blockIdx.x / p.parts, start = blockIdx.x % p.parts * p.span;
   RowSpace& w = p.space[r];
   const Settings o(a, r);
-  if (o.few(PART_K, false)) return;
+  if (!summed_in_parts(o)) return;
   const Whole whole(w, p.parts);
-  if (!drawn_in_parts(o, whole)) return;
+  if (whole.there <= CAP<THREADS>) return;
   const Row row(o.temperature, key_score(whole.most), fraction_bits(a.columns));
   const Bins bins = bins_of(row, whole);
   for (uint32_t i = threadIdx.x; i < BINS; i += SHORT_THREADS) {
@@ -1443,7 +1444,7 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void collect_kernel(DrawArgs a, P
   const uint32_t r = blockIdx.x / p.parts, part = blockIdx.x % p.parts, start = part * p.span, tid = threadIdx.x;
   RowSpace& w = p.space[r];
   const Settings o(a, r);
-  if (o.few(PART_K, false)) return;
+  if (!summed_in_parts(o)) return;
   // what does not depend on one another is asked for at once: the kernel is a chain of waits
   uint64_t mine[PER], sum = 0, total;  // the thread's bins
   uint32_t counts[PER];
@@ -1453,7 +1454,7 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void collect_kernel(DrawArgs a, P
   for (uint32_t i = 0; i < PER; ++i) counts[i] = w.count[PER * tid + i];
   const double u = uniform_of(a, r);
   const Whole whole(w, p.parts);
-  if (!drawn_in_parts(o, whole)) return;
+  if (whole.there <= CAP<THREADS>) return;
   const Row row(o.temperature, key_score(whole.most), fraction_bits(a.columns));
   const Bins bins = bins_of(row, whole);
   const float z_least = o.min_p > 0.0f ? least_of_min_p(row, o.min_p, whole.most) : 0.0f;
@@ -1554,7 +1555,7 @@ __device__ __forceinline__ bool draw_collected(Shared<THREADS>& s, const RowSpac
     *d = nothing_to_draw();
     return true;
   }
-  if (!drawn_in_parts(o, whole) || n > CAP<THREADS>) return false;
+  if (whole.there <= CAP<THREADS> || n > CAP<THREADS>) return false;
   const Row row(o.temperature, key_score(whole.most), fraction_bits(columns));
   const Bins bins = bins_of(row, whole);
   uint64_t* const list = s.large.some.l.list;
@@ -1630,22 +1631,25 @@ __device__ __forceinline__ bool draw_collected(Shared<THREADS>& s, const RowSpac
 // k entries up to the last of them: what comes after that one is not among the k best.
 __device__ __forceinline__ bool draw_joined(ListShared<THREADS>& s, const RowSpace& w, uint32_t parts, const Settings& o, double u, Result* d) {
   constexpr int BT = THREADS;
+  static_assert(MAX_PARTS * PART_K == 2 * BT && 2 * BT <= CAP<BT> && PART_K % 64 == 0, "two entries a thread, a wavefront in one list at a time");
   const uint32_t lane = threadIdx.x & 63, k = o.greedy() ? 1 : o.top_k, j = (k + parts - 1) / parts;
-  const uint32_t count = lane < parts ? w.part_count[lane] : 0;
-  uint64_t last = lane >= parts ? 0 : count >= j && count != MANY_EQUAL ? w.part_list[lane][j - 1] : LIST_END;
+  // everything is asked for at once; beyond the parts and their counts it is whatever was there
+  const uint32_t n = w.part_count[lane % MAX_PARTS], count = lane < parts ? n : 0;
+  const uint64_t jth = w.part_list[lane % MAX_PARTS][j - 1];
+  uint64_t e[2];
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) e[i] = w.part_list[(i * BT + threadIdx.x) / PART_K][threadIdx.x % PART_K];
   if (threadIdx.x == 0) s.n = 0;
   if (__ballot(count == MANY_EQUAL)) return false;  // every wavefront sees the same counts
+  uint64_t last = lane >= parts ? 0 : count >= j ? jth : LIST_END;
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) last = max(last, shfl_xor_u64(last, m));
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < parts * PART_K; i += BT) {
-    const uint32_t n = (uint32_t)__shfl((int)count, (int)(i / PART_K), 64);
-    if (i % PART_K < n) {
-      const uint64_t e = w.part_list[i / PART_K][i % PART_K];
-      if (e <= last) s.list[atomicAdd(&s.n, 1u)] = e;
-    }
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) {
+    const uint32_t entries = (uint32_t)__shfl((int)count, (int)((i * BT + threadIdx.x) / PART_K), 64);
+    if (threadIdx.x % PART_K < entries && e[i] <= last) s.list[atomicAdd(&s.n, 1u)] = e[i];
   }
-  static_assert(MAX_PARTS * PART_K <= CAP<BT> && PART_K % 64 == 0, "all lists at once, a wavefront in one of them");
   __syncthreads();
   const uint32_t m = s.n;
   *d = !m ? nothing_to_draw() : o.greedy() ? first_listed(s, m) : draw_list(s, m, o, u);
@@ -1665,7 +1669,10 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(DrawArgs a, bool left, Pa
   bool done = false;
   if constexpr (PARTS) {
     const RowSpace& w = p.space[r];
-    done = o.few(PART_K, false) ? draw_joined(s.large.some.l, w, p.parts, o, u, &d) : draw_collected(s, w, p.parts, a.columns, o, u, &d);
+    if (listed_in_parts(o))
+      done = draw_joined(s.large.some.l, w, p.parts, o, u, &d);
+    else if (summed_in_parts(o))
+      done = draw_collected(s, w, p.parts, a.columns, o, u, &d);
     __syncthreads();
   }
   if (!done) d = draw_row<T, THREADS>((const T*)a.logits + r * a.stride, a.columns, s, o, u);
@@ -1739,7 +1746,7 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void draw_short_kernel(DrawArgs a
 constexpr uint32_t SHORT_ROW_16 = 20480, SHORT_ROW_32 = 32768, MANY_ROWS = 256;
 // Parts of a row: two workgroups a CU, of at least 4,096 columns each, eight and more.  What rows of few candidates lose is the launches of
 // kernels that have nothing to do with them.  (us, a workgroup a row / in parts, fp32: 8 x 131,072 by top-p 114 / 48, top-k of 50
-// 19 / 21; 40 x 100,003 by top-p 95 / 49, top-k of 40 19 / 22; 128 x 100,003, by four, 107 / 95 and 27 / 31.  16-bit rows, whose values are
+// 19 / 21, of 400 34 / 42; 40 x 100,003 by top-p 95 / 50, top-k of 40 19 / 22; 128 x 100,003, by four, 107 / 95 and 27 / 31.  16-bit rows, whose values are
 // counted: 65,536 by top-k of 50 11 / 17.)
 Parts parts_of(size_t size, uint32_t rows, uint32_t columns, void* workspace) {
   Parts p{};
