@@ -293,7 +293,7 @@ int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, uint32_t col
  * At most 2^26 columns (SKY_ERR_LIMIT).
  * workspace: sky_logits_draw_workspace says how many bytes a draw of such a matrix can make use of (0: none), aligned to 16; nothing need
  * be in them, two calls that may run at the same time have one workspace each, and a captured graph keeps its own.  With it several
- * workgroups share each of a few long fp32 rows; NULL: every row is drawn from by one workgroup, the same ids, later. */
+ * workgroups share each of a few long fp32 rows; NULL: every row is drawn from by one workgroup.  The ids are the same. */
 typedef struct sky_draw_rules {
   const float* temperature;
   const uint32_t* top_k;

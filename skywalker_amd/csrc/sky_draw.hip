@@ -1290,6 +1290,7 @@ __device__ __forceinline__ float least_of_min_p(const Row& row, float min_p, uin
   }
   return P::value(min(lo + 1, most));
 }
+
 __global__ __launch_bounds__(SHORT_THREADS, 4) void parts_kernel(DrawArgs a, Parts p) {
   constexpr int BT = SHORT_THREADS;
   using T = float;

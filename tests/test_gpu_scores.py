@@ -192,10 +192,11 @@ def run_draw(capi, orc, x, dtype, pad=0, lead=0, t=None, top_k=None, top_p=None,
     logprobs, kept = dev(capi, np.full(rows + 1, 5.0), np.float32), dev(capi, np.full(rows + 1, 777), np.uint32)
     need = capi.logits_draw_workspace(code(capi, dtype), rows, columns)
     results = []
-    for ws in ([None, capi.DeviceArray(max(need, 16), np.uint8)] if workspace else [None]):
+    for ws in ([None, dev(capi, np.full(need + 16, 255), np.uint8)] if workspace else [None]):  # nothing need be in it
         capi.logits_draw(m, code(capi, dtype), rows, columns, rules, tokens, uniforms=dev(capi, u, np.float64), seed=seed, first_walker=first,
                          step=step, logprobs=logprobs, kept=kept, row_stride=m.stride, tokens_stride=stride, workspace=ws)
         capi.synchronize()
+        assert ws is None or (ws.to_host()[need:] == 255).all()
         results.append((tokens.to_host(), logprobs.to_host(), kept.to_host()))
     for tok, lp, kp in results:
         assert (tok[rows * stride:] == 777).all() and lp[rows] == 5.0 and kp[rows] == 777
@@ -547,9 +548,10 @@ class Hip:
         return s
 
 
-def test_scores_on_a_stream_and_in_a_graph(capi):
+@pytest.mark.parametrize("columns", [5003, 40003])  # a workgroup a row, and rows in parts
+def test_scores_on_a_stream_and_in_a_graph(capi, columns):
     rng = np.random.default_rng(14)
-    rows, columns, E = 24, 5003, 100
+    rows, E = 24, 100
     hip = Hip()
     x, r_in = Matrix(capi, rng.normal(0, 3, (rows, columns)), "f32"), Matrix(capi, rng.normal(0, 2, (rows, E)), "f32")
     rules = capi.LogitsRules(history=dev(capi, rng.integers(0, columns, (rows, 90)), np.uint32), history_columns=90,

@@ -76,6 +76,8 @@ def test_draw_refusals(capi):
     refused(capi, LIMIT, "2^31", draw, x, capi.F16, 1, 1 << 31, None, t)
     refused(capi, LIMIT, "too large", draw, x, capi.F16, 1 << 30, 8, None, t, row_stride=1 << 40)
     assert capi.lib().sky_logits_draw_workspace(0, 1, 1, None) == ARG
+    need = capi.logits_draw_workspace(capi.F32, 3, 100000)
+    refused(capi, ARG, "too small", draw, x, capi.F32, 3, 100000, None, t, workspace=Fake(4096), workspace_bytes=need - 1)
 
 
 def test_route_refusals(capi):
