@@ -869,12 +869,14 @@ extern "C" int sky_route_topk(const void* logits, int dtype, uint32_t rows, uint
   a.counts = counts;
   uint32_t slots = 1;
   while (slots < rules->k) slots *= 2;
-  // Experts of fewer lanes than k leave the quads without a k-th largest: all that may be chosen are candidates, more than are listed, and
-  // every row is chosen from one by one (7 x 203 by the 14 best, of 13 lanes: 63 us, a row a wavefront 8; 20,000 x 203 141 and 39).
+  // Where k lanes of experts are all there are, the least of the lanes' largest lets in many, and where there are fewer, all that may be
+  // chosen are candidates, more than are listed, and every row is chosen from one by one.  (us, quads / a row a wavefront: 203 experts
+  // by the 14 best, 13 lanes, 7 rows 63 / 8, 20,000 rows 141 / 39, by the 13 best 58 / 50; 256 by the 16 best, 16 lanes, 75 / 56, by
+  // the 14 best 39 / 51, by the 9 best 28 / 39.)
   uint32_t per = 1;
   while (16 * per < experts) per *= 2;
   const uint32_t open = experts / rules->groups * rules->groups_kept;
-  const bool listed = open <= QUAD_LISTED || rules->k <= (open + per - 1) / per;
+  const bool listed = open <= QUAD_LISTED || rules->k < (open + per - 1) / per;
   if (experts <= QUAD_EXPERTS && rules->k <= QUAD_K && rules->groups <= QUAD_GROUPS && listed) {
     // four rows at a time, as many times as fill the wavefront with chosen experts, as long as there are wavefronts for every SIMD
     slots = std::max(slots, 4u);

@@ -391,7 +391,7 @@ def run_route(capi, x, dtype, k, pad=0, lead=0, counts=True, **kw):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows,E,k", [(1, 1, 1), (5, 8, 2), (3, 64, 64), (9, 100, 6), (130, 65, 3), (7, 256, 8), (4, 500, 16), (3, 1024, 33)])
+@pytest.mark.parametrize("rows,E,k", [(1, 1, 1), (5, 8, 2), (3, 64, 64), (9, 100, 6), (130, 65, 3), (7, 256, 8), (7, 203, 14), (5, 203, 13), (6, 203, 12), (3, 256, 16), (4, 500, 16), (3, 1024, 33)])
 @pytest.mark.parametrize("sigmoid", [False, True])
 def test_route_follows_its_definition(capi, dtype, rows, E, k, sigmoid):
     rng = np.random.default_rng(E * 7 + k)
