@@ -389,7 +389,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
       bool stays = mine && larger16<false>(mine, sub) < a.r.groups_kept;
       if (__ballot((uint32_t)__popc((uint32_t)(__ballot(stays) >> (lane & 48)) & 0xFFFFu) > a.r.groups_kept)) stays = mine && larger16<true>(mine, sub) < a.r.groups_kept;  // equal ones
       const uint32_t last = min16(stays ? mine : 0xFFFFFFFFu), next = max16(stays ? 0 : mine);
-      if (!by_logit && next) doubt = !(key_score(last) - key_score(next) > 3.0f * near);
+      if (!by_logit && next) doubt |= !(key_score(last) - key_score(next) > 3.0f * near);  // (of a NaN among the biases `near` knows nothing)
       const uint32_t stay = (uint32_t)(__ballot(stays) >> (lane & 48)) & 0xFFFFu;
       if (whole_lanes) {
         const bool mine_stays = stay >> owner & 1;
