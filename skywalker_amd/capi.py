@@ -402,13 +402,17 @@ def _addr(a):
 
 
 class _Rules(C.Structure):
-    """A rules struct that is built once and used for many calls; it keeps the arrays that it points to."""
+    """A rules struct that is built once and used for many calls; it keeps the arrays that it points to as long as it lives, which
+    is as long as a captured call is replayed."""
 
     def _point(self, arrays):
         self._arrays = arrays
         for name, a in arrays.items():
             setattr(self, name, _addr(a))
-        self.ref = C.byref(self)
+
+    @property
+    def ref(self):  # not kept: it holds the struct, and such a circle is never collected
+        return C.byref(self)
 
 
 class LogitsRules(_Rules):
