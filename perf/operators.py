@@ -183,10 +183,10 @@ def _inputs(case, seed):
 
 
 class _Buffer:
-    """A torch tensor where capi takes one of its own arrays: anything with the address under `ptr`."""
+    """A torch tensor where capi takes one of its own arrays: anything with the address under `ptr`, and the size of a workspace."""
 
     def __init__(self, tensor):
-        self.tensor, self.ptr = tensor, ctypes.c_void_p(tensor.data_ptr())
+        self.tensor, self.ptr, self.nbytes = tensor, ctypes.c_void_p(tensor.data_ptr()), tensor.nbytes
 
 
 def prepare(case, seed):
