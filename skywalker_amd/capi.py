@@ -6,6 +6,7 @@ and every call fails loudly when no MI355X is visible.
 """
 import ctypes as C
 import os
+import warnings
 
 import numpy as np
 
@@ -470,11 +471,15 @@ def logits_draw_workspace(dtype, rows, columns):
 
 def logits_draw(logits, dtype, rows, columns, rules, tokens, uniforms=None, seed=0, first_walker=0, step=0, logprobs=None, kept=None,
                 row_stride=0, tokens_stride=0, workspace=None, workspace_bytes=None, stream=None):
-    """sky_logits_draw.  workspace_bytes None: as many as logits_draw_workspace asks for."""
+    """sky_logits_draw.  workspace_bytes None: the workspace's `nbytes`; one that does not tell its size is not made use of."""
     if workspace is None:
         workspace_bytes = 0
     elif workspace_bytes is None:
-        workspace_bytes = logits_draw_workspace(dtype, rows, columns)
+        workspace_bytes = getattr(workspace, "nbytes", None)
+        if workspace_bytes is None:
+            if logits_draw_workspace(dtype, rows, columns):
+                warnings.warn("logits_draw: a workspace without nbytes is not made use of: give workspace_bytes", RuntimeWarning, 2)
+            workspace, workspace_bytes = None, 0
     _ck(lib().sky_logits_draw(_addr(logits), dtype, rows, columns, row_stride, rules.ref if rules is not None else None, _addr(uniforms),
                               seed, first_walker, step, _addr(tokens), tokens_stride, _addr(logprobs), _addr(kept), _addr(workspace),
                               workspace_bytes, stream))
