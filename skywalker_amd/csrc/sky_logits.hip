@@ -284,11 +284,14 @@ __global__ __launch_bounds__(NEAR_THREADS) void adjust_near_kernel(AdjustArgs a)
   const Sparse sparse(a, row);
   uint32_t id[EACH], slot[EACH];
   float value[EACH];
+  // Every element is written once: of `if (...) id[i] = SKY_INVALID` behind the loads the compiler (ROCm 7.2) kept the first element's
+  // write alone, and masks did not reach the others.
 #pragma unroll
   for (uint32_t i = 0; i < EACH; ++i) {
-    const uint32_t j = lo + tid + i * NEAR_THREADS;
-    id[i] = j < hi ? a.adjncy[j] : SKY_INVALID;
-    if (id[i] >= a.columns || (mask && !(mask[id[i] >> 5] >> (id[i] & 31) & 1u))) id[i] = SKY_INVALID;
+    const uint32_t j = lo + tid + i * NEAR_THREADS, v = j < hi ? a.adjncy[j] : SKY_INVALID;
+    uint32_t bits = v < a.columns ? 1u : 0u;
+    if (mask && bits) bits = mask[v >> 5] >> (v & 31);
+    id[i] = bits & 1u ? v : SKY_INVALID;
   }
 #pragma unroll
   for (uint32_t i = 0; i < EACH; ++i) value[i] = id[i] != SKY_INVALID ? (float)x[id[i]] : 0.0f;

@@ -2,9 +2,72 @@
 import numpy as np
 import pytest
 
-from test_gpu_scores import INF, capi, run_route  # noqa: F401  (capi is a fixture)
+import scores_oracle as so
+import test_gpu_scores as base
+from test_gpu_scores import INF, INVALID, Matrix, capi, dev, run_adjust, run_route, some_rules  # noqa: F401  (capi is a fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def place_by_place(monkeypatch):
+    """Infinities and NaN are compared place by place: what is wanted to be -inf is, and nothing else."""
+    def near(got, want, error, dtype):
+        gone = ~np.isfinite(want)
+        assert np.array_equal(got[gone], want[gone], equal_nan=True)
+        assert np.isfinite(got[~gone]).all()
+        numbers(got, want, error, dtype)
+
+    numbers = base.near
+    monkeypatch.setattr(base, "near", near)
+
+
+# ------------------------------------------------------------------------------------------------ adjust
+def with_odd_values(rng, x):
+    """Some NaN and infinities among the logits."""
+    at = rng.random(x.shape)
+    return np.where(at < 0.01, np.nan, np.where(at < 0.02, INF, np.where(at < 0.03, -INF, x))).astype(np.float32)
+
+
+def test_the_comparison_tells_infinities_apart():
+    z = np.zeros(2)
+    for got, want in (([5.0, 1.0], [-INF, 1.0]), ([INF, 1.0], [-INF, 1.0]), ([-INF, 1.0], [1.0, 1.0]), ([np.nan, 1.0], [-INF, 1.0]), ([1.0, 1.0], [np.nan, 1.0])):
+        with pytest.raises(AssertionError):
+            base.near(np.array(got), np.array(want), z, "f32")
+    base.near(np.array([-INF, 1.0]), np.array([-INF, 1.0]), z, "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,columns,history,biases,masks", [
+    (1, 1, 1, 1, 1), (4, 1025, 0, 0, 3), (9, 8191, 300, 20, 2), (5, 20011, 3001, 5000, 4), (6, 8193, 0, 0, 1), (40, 70, 9, 5, 40)])
+def test_adjusted_rows_place_by_place(capi, dtype, rows, columns, history, biases, masks):  # noqa: F811
+    rng = np.random.default_rng(rows * 1000033 + columns)
+    x = with_odd_values(rng, rng.normal(0, 4, (rows, columns)))
+    kw = some_rules(rng, rows, columns, history, biases, masks)
+    for pad, out_pad, lead, in_place in ((0, 0, 0, False), (3, 5, 1, False), (7, 0, 3, True)):
+        run_adjust(capi, x, dtype, pad, out_pad, lead, in_place, **kw)
+
+
+DEGREES = [0, 1, 255, 256, 257, 300, 511, 512, 513, 768, 769, 1000, 1023, 1024, 1025, 1300, 5000]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_adjust_by_a_graph_with_rows_of_every_length(capi, dtype, in_place):  # noqa: F811
+    # a workgroup has up to four neighbours a thread in its table; rows of more than 1,024 are done tile by tile
+    rng = np.random.default_rng(17)
+    V, n = 9001, len(DEGREES)
+    xadj = np.concatenate([[0], np.cumsum(DEGREES), np.full(V - n, sum(DEGREES))]).astype(np.uint32)
+    adjncy = np.concatenate([rng.permutation(V)[:d] if i % 2 else rng.integers(0, V, d) for i, d in enumerate(DEGREES)]).astype(np.uint32)  # none sorted, half with repetitions
+    g = capi.Graph.upload(xadj, adjncy, None)
+    states = np.concatenate([rng.permutation(n), [V, INVALID, V - 1]]).astype(np.uint32)
+    rows = len(states)
+    for columns, stride in ((V, 1), (V - 333, 9), (V + 777, 1)):
+        x = with_odd_values(rng, rng.normal(0, 4, (rows, columns)))
+        for rules in ((0, 0, 0), (81, 0, 0), (300, 40, 3), (0, 2500, 2)):
+            for pad, lead in ((0, 0), (3, 1)):
+                run_adjust(capi, x, dtype, pad, 2 * pad, lead, in_place, g=g, stride_of=stride, xadj=xadj, adjncy=adjncy, states=states, **some_rules(rng, rows, columns, *rules))
+    g.free()
 
 
 # ------------------------------------------------------------------------------------------------ route
