@@ -308,7 +308,10 @@ int sky_logits_draw(const void* logits, int dtype, uint32_t rows, uint32_t colum
 
 /* The k best experts of every row.  score = softmax or sigmoid of the row's logits; experts compete by score + bias (bias[e],
  * NULL: none), equal ones by their number.  With groups > 1 the experts form `groups` ranges of the same length, of which
- * the groups_kept best stay: a group is worth its best expert, or its two best together (group_top2).  ids[r * k + j] receives
+ * the groups_kept best stay: a group is worth its best expert, or its two best together (group_top2).  Where nothing is added to a score
+ * (bias NULL, and no groups that are compared by their two best) the logits themselves are compared, with which both scores ascend; else
+ * sums in fp64, in which scores may be equal whose logits are not (sigmoids of 37 and more are 1): those go by their number, with a bias of
+ * zeros as with any other.  ids[r * k + j] receives
  * the j-th best, weights[r * k + j] scale * score, with `renormalise` divided by the sum of the row's k scores; the bias has
  * no part in the weights.  A logit of NaN or -inf closes an expert: it is not chosen, and places that find no open expert receive
  * SKY_INVALID with weight 0; +inf counts as the largest number.  A bias of NaN or -inf closes its expert for all rows, one of +inf puts

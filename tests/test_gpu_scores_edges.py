@@ -86,3 +86,15 @@ def test_route_by_groups_with_one_bias_that_is_no_finite_number(capi, sigmoid, E
             for top2 in (False, True):
                 ids = run_route(capi, x, "f32", k, sigmoid=sigmoid, bias=b, groups=groups, kept=kept, top2=top2, renormalise=not top2)
                 assert (ids == at).any(axis=1).all() if odd == INF else not (ids == at).any()
+
+
+@pytest.mark.parametrize("E,groups,kept,top2", [(64, 1, 1, False), (300, 1, 1, False), (64, 4, 2, True), (512, 4, 2, True)])
+def test_route_of_scores_that_are_equal_in_64_bits(capi, E, groups, kept, top2):  # noqa: F811
+    # sigmoids of 40 and more are 1: by the logits themselves where nothing is added to a score, by their sums else
+    x = np.full((2, E), -3.0, np.float32)
+    x[0, [9, 20, 31]] = [40.0, 60.0, 50.0]
+    x[1, [9, 20, 31]] = [50.0, 40.0, 60.0]
+    ids = run_route(capi, x, "f32", 3, sigmoid=True, groups=groups, kept=kept, top2=top2)
+    assert ids.tolist() == ([[20, 31, 9], [31, 9, 20]] if not top2 else [[9, 20, 31]] * 2)
+    for b in (np.zeros(E, np.float32), np.full(E, 0.25, np.float32)):
+        assert run_route(capi, x, "f32", 3, sigmoid=True, bias=b, groups=groups, kept=kept, top2=top2).tolist() == [[9, 20, 31]] * 2
