@@ -2,8 +2,8 @@
 //   score    s_e = exp(x_e - max) / sum, or 1 / (1 + exp(-x_e))
 //   choice   by s_e + b_e, the largest first, equal ones by number.  Both scores ascend with the logit, so without a bias and
 //            without pairs of experts the choice goes by the logits themselves, exactly.  Else it is made from scores in fp32, whose error
-//            has a bound; where two of those that it hangs on (neighbours among the k + 1 best, the last group that stays and the first
-//            that does not) are nearer than that and not alike, the row is chosen again in fp64: one expert more or less is no
+//            has a bound; where two of those that it hangs on (neighbours among the k + 1 best, what is as near to the last of them, the last group that stays and the
+//            first that does not) are nearer than that and not alike, the row is chosen again in fp64: one expert more or less is no
 //            rounding error.  (32,768 rows of 256, 8 of 4 of 8 groups: all in fp64 96 us.)
 //   weights  w_j = scale * s_j, renormalised scale * s_j / sum of the k chosen.  Renormalised, the sum over all experts drops out of
 //            softmax scores, and sigmoid scores are taken relative to the largest of the chosen (their logarithms
@@ -101,6 +101,12 @@ __device__ __forceinline__ double exp_negative(double x) {
 __device__ __forceinline__ double sigmoid_over(double x, double m) { return exp_negative(fmin(x, 0.0) - m) / (1.0 + exp_negative(-fabs(x))); }
 
 __device__ __forceinline__ bool chosen_by_logit(const sky_route_rules& r) { return !r.bias && !(r.groups > 1 && r.groups_kept < r.groups && r.group_top2); }
+
+// Whether two experts of a row have the same logit and bias: the same score then, and they stand by number.
+template <typename T>
+__device__ __forceinline__ bool alike(const RouteArgs& a, const T* x, uint32_t e, uint32_t f) {
+  return (float)x[e] == (float)x[f] && (!a.r.bias || a.r.bias[e] == a.r.bias[f]);
+}
 
 // The choice of one row in fp64, into lanes first + j.  Keys: 0 is a closed expert, a taken one or none.
 template <typename T, int PER>
@@ -448,10 +454,21 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES, 4) void route_quad_kernel(RouteAr
     }
     __builtin_amdgcn_wave_barrier();
     // (best[listed] is -inf, further than any bound from a finite number: place[listed], which is not set, is then not looked at)
+    bool level = false;  // the last that is chosen and the first that is not are alike
     if (!by_logit && !odd && sub < k && sub < listed && !(s.best[quarter][sub] - s.best[quarter][sub + 1] > near)) {
       // alike, the same logit and bias, they stand as they are
-      const uint32_t e = s.place[quarter][sub], f = s.place[quarter][sub + 1];
-      doubt |= !((float)x[e] == (float)x[f] && (!a.r.bias || a.r.bias[e] == a.r.bias[f]));
+      const uint32_t e = s.place[quarter][sub];
+      const bool same = alike(a, x, e, s.place[quarter][sub + 1]);
+      doubt |= !same;
+      level = same && sub == k - 1;
+    }
+    // then one behind them that is as near may be better than both: all of these have to be alike
+    const uint64_t levels = __ballot(level);
+    if (levels >> (lane & 48) & 0xFFFFu) {
+      const float v = s.best[quarter][k - 1];
+      const uint32_t e = s.place[quarter][k - 1];
+      for (uint32_t c = sub; c < listed; c += 16)
+        if (!(fabsf(v - s.listed[quarter][c]) > near)) doubt |= !alike(a, x, e, s.expert[quarter][c]);
     }
     // rows in doubt, one after another by the whole wavefront
     uint64_t rest = __ballot(doubt);
@@ -623,9 +640,16 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_kernel(RouteArgs a, ui
       if (!best) break;
       const uint32_t winner = (uint32_t)__builtin_ctzll(__ballot(mine == best));  // of equals the first lane, and its first, has the smallest number
       const uint32_t e = (uint32_t)__builtin_amdgcn_readlane((int)(lane * PER + at), (int)winner);
-      if (!by_logit && j && !(key_score(before) - key_score(best) > near))
-        // alike: the same logit and bias
-        exact = (float)x[e] == (float)x[before_e] && (!a.r.bias || a.r.bias[e] == a.r.bias[before_e]);
+      if (!by_logit && j && !(key_score(before) - key_score(best) > near)) {
+        exact = alike(a, x, e, before_e);
+        if (exact && j == k) {  // one behind them that is as near may be better than both: all of these have to be alike
+          bool other = false;
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (key[i] && !(key_score(before) - key_score(key[i]) > near)) other |= !alike(a, x, before_e, lane * PER + i);
+          exact = __ballot(other) == 0;
+        }
+      }
       before = best;
       before_e = e;
 #pragma unroll

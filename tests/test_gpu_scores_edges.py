@@ -98,3 +98,19 @@ def test_route_of_scores_that_are_equal_in_64_bits(capi, E, groups, kept, top2):
     assert ids.tolist() == ([[20, 31, 9], [31, 9, 20]] if not top2 else [[9, 20, 31]] * 2)
     for b in (np.zeros(E, np.float32), np.full(E, 0.25, np.float32)):
         assert run_route(capi, x, "f32", 3, sigmoid=True, bias=b, groups=groups, kept=kept, top2=top2).tolist() == [[9, 20, 31]] * 2
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("E,groups,kept", [(24, 1, 1), (100, 1, 1), (256, 8, 3), (203, 1, 1), (288, 32, 21), (700, 1, 1), (1024, 4, 2)])
+def test_route_past_pairs_of_equal_experts(capi, sigmoid, E, groups, kept):  # noqa: F811
+    # scores that fp32 cannot tell apart and fp64 can: the last that is chosen and the first that is not are often the same, and a better one stands behind
+    rng = np.random.default_rng(E * 13 + groups)
+    if sigmoid:
+        x = rng.choice(np.float32([24, 24.5, 26, 30, 17, 2]), (90, E), p=[0.3, 0.2, 0.02, 0.01, 0.37, 0.1])
+    else:
+        x = np.float32(1.0) + rng.choice(np.float32([0, 1, 2, 3, -2.0 ** 22]), (90, E), p=[0.6, 0.05, 0.03, 0.02, 0.3]) * np.float32(2.0 ** -23)
+    x[80:] = x[80:, :1]  # all of a row the same
+    x[:, :(groups - kept) * (E // groups)] = -9.0  # groups that are worth less, beyond doubt
+    for k in (1, 2, 3, 8, 13, 16):
+        for b in (np.zeros(E, np.float32), np.full(E, 0.25, np.float32)):
+            run_route(capi, x, "f32", k, sigmoid=sigmoid, bias=b, groups=groups, kept=kept, top2=k % 2 == 1)
