@@ -279,7 +279,8 @@ int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, uint32_t col
                       const sky_logits_rules* rules, void* out, uint64_t out_stride, void* stream);
 
 /* One id of every row by chance.  Entries are ordered by logit, largest first, equal ones by column, and weigh
- * exp((logit - largest) / temperature).  NaN and -inf are not there to be drawn; +inf counts as the largest number.
+ * exp((logit - largest) / temperature).  NaN and -inf are not there to be drawn; +inf counts as the largest number of the logits' type
+ * (65,504 of SKY_F16).
  *   temperature[r]  NULL: 1; not above 0: the first entry of the order is taken
  *   top_k[r]        only the first top_k of the order stay (0, NULL: all)
  *   top_p[r]        only the shortest beginning of the order whose weight is at least top_p of what top_k left, the first entry in
@@ -314,7 +315,7 @@ int sky_logits_draw(const void* logits, int dtype, uint32_t rows, uint32_t colum
  * zeros as with any other.  ids[r * k + j] receives
  * the j-th best, weights[r * k + j] scale * score, with `renormalise` divided by the sum of the row's k scores; the bias has
  * no part in the weights.  A logit of NaN or -inf closes an expert: it is not chosen, and places that find no open expert receive
- * SKY_INVALID with weight 0; +inf counts as the largest number.  A bias of NaN or -inf closes its expert for all rows, one of +inf puts
+ * SKY_INVALID with weight 0; +inf counts as the largest fp32 number.  A bias of NaN or -inf closes its expert for all rows, one of +inf puts
  * it before the others.  counts[e] (may be NULL) receives how often expert e was chosen
  * (0 for all when there are no rows).
  * At most 1,024 experts, k of at most 64, at most 64 groups, at most 2^25 rows (SKY_ERR_LIMIT).

@@ -4,7 +4,7 @@ import pytest
 
 import scores_oracle as so
 import test_gpu_scores as base
-from test_gpu_scores import INF, INVALID, Matrix, capi, dev, run_adjust, run_route, some_rules  # noqa: F401  (capi is a fixture)
+from test_gpu_scores import INF, INVALID, Matrix, capi, dev, run_adjust, run_draw, run_route, some_rules  # noqa: F401  (capi is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -68,6 +68,27 @@ def test_adjust_by_a_graph_with_rows_of_every_length(capi, dtype, in_place):  # 
             for pad, lead in ((0, 0), (3, 1)):
                 run_adjust(capi, x, dtype, pad, 2 * pad, lead, in_place, g=g, stride_of=stride, xadj=xadj, adjncy=adjncy, states=states, **some_rules(rng, rows, columns, *rules))
     g.free()
+
+
+# ------------------------------------------------------------------------------------------------ draw
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_draw_from_rows_without_columns(capi, dtype):  # noqa: F811
+    tokens, logprobs, kept = dev(capi, np.full(3, 777), np.uint32), dev(capi, np.full(3, 5.0), np.float32), dev(capi, np.full(3, 777), np.uint32)
+    capi.logits_draw(None, base.code(capi, dtype), 3, 0, None, tokens, logprobs=logprobs, kept=kept)
+    assert tokens.to_host().tolist() == [INVALID] * 3 and logprobs.to_host().tolist() == [-INF] * 3 and kept.to_host().tolist() == [0] * 3
+
+
+@pytest.mark.parametrize("dtype,largest", [("f32", float(np.finfo(np.float32).max)), ("f16", 65504.0), ("bf16", 3.3895313892515355e38)])
+@pytest.mark.parametrize("columns", [70, 5000, 40007])
+def test_draw_counts_infinity_as_the_largest_number_of_the_type(capi, orc, monkeypatch, dtype, largest, columns):  # noqa: F811
+    monkeypatch.setattr(so, "BIG", largest)
+    rng = np.random.default_rng(columns)
+    x = (rng.normal(0, 0.2, (6, columns)) * largest).clip(-largest, largest).astype(np.float32)
+    x[:, [3, 50]], x[:, [7, 20]] = INF, largest
+    x[4:, 3::2] = INF
+    for t in (largest, largest / 50, 1e-3):
+        run_draw(capi, orc, x, dtype, pad=1, t=np.full(6, t), u=rng.random(6), workspace=True)
+        run_draw(capi, orc, x, dtype, t=np.full(6, t), top_k=np.array([0, 3, 40, columns // 2, 700, 1]), top_p=np.full(6, 0.9), min_p=np.full(6, 0.01), u=rng.random(6), workspace=True)
 
 
 # ------------------------------------------------------------------------------------------------ route
