@@ -1,4 +1,6 @@
 """Choices from rows of scores on the GPU: settings at their borders, against the definitions in 64 bits (scores_oracle)."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -70,6 +72,32 @@ def test_adjust_by_a_graph_with_rows_of_every_length(capi, dtype, in_place):  # 
     g.free()
 
 
+@pytest.mark.parametrize("by_graph", [False, True])
+def test_adjust_takes_a_prefix_of_the_paths_as_history(capi, by_graph):  # noqa: F811
+    # what of a row of paths lies behind history_columns does not count, whatever it is
+    rng = np.random.default_rng(23)
+    rows, V, have, stride = 20, 3000, 31, 81
+    paths = rng.integers(0, 40, (rows, stride)).astype(np.uint32)
+    x = rng.normal(0, 3, (rows, V)).astype(np.float32)
+    xadj, adjncy = (np.arange(V + 1) * 20).astype(np.uint32), rng.integers(0, 60, V * 20, dtype=np.uint32)
+    g = capi.Graph.upload(xadj, adjncy, None) if by_graph else None
+    column = dev(capi, paths, np.uint32)
+    rep, frequency = rng.uniform(1, 1.5, rows).astype(np.float32), rng.uniform(0, 1, rows).astype(np.float32)
+
+    class Last:
+        ptr = column.ptr.value + 4 * (have - 1)
+
+    m, out = Matrix(capi, x, "f32"), Matrix(capi, x, "f32", 3)
+    rules = capi.LogitsRules(history=column, history_columns=have, history_stride=stride, repetition=dev(capi, rep, np.float32), frequency=dev(capi, frequency, np.float32),
+                             graph=g, states=Last if by_graph else None, states_stride=stride if by_graph else 0)
+    capi.logits_adjust(m, capi.F32, rows, V, rules, out, out_stride=out.stride)
+    held = dict(xadj=xadj, adjncy=adjncy, states=paths[:, have - 1]) if by_graph else {}
+    want, error = so.adjust(m.values, history=paths[:, :have], rep=rep, frequency=frequency, **held)
+    base.near(out.read(), want, error, "f32")
+    if g:
+        g.free()
+
+
 # ------------------------------------------------------------------------------------------------ draw
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_draw_from_rows_without_columns(capi, dtype):  # noqa: F811
@@ -89,6 +117,29 @@ def test_draw_counts_infinity_as_the_largest_number_of_the_type(capi, orc, monke
     for t in (largest, largest / 50, 1e-3):
         run_draw(capi, orc, x, dtype, pad=1, t=np.full(6, t), u=rng.random(6), workspace=True)
         run_draw(capi, orc, x, dtype, t=np.full(6, t), top_k=np.array([0, 3, 40, columns // 2, 700, 1]), top_p=np.full(6, 0.9), min_p=np.full(6, 0.01), u=rng.random(6), workspace=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_draw_from_the_longest_rows(capi, dtype):  # noqa: F811
+    # 2^26 columns of one value, and of one in three: the units of 2^26 weights stay below 2^62
+    n = 1 << 26
+    bits = np.zeros(n, so.storage(dtype))
+    need = capi.logits_draw_workspace(base.code(capi, dtype), 1, n)
+    tokens, logprobs, kept = capi.DeviceArray(1, np.uint32), capi.DeviceArray(1, np.float32), capi.DeviceArray(1, np.uint32)
+    for third in (False, True):
+        if third:
+            bits[:] = so.to_bits(np.full(1, -INF, np.float32), dtype)[0]
+            bits[1::3] = 0
+        there = np.count_nonzero(bits == 0)
+        m = capi.DeviceArray.from_host(bits)
+        for ws in [None] + ([capi.DeviceArray(need, np.uint8)] if need else []):
+            for u, k in ((0.0, 0), (0.3, 0), (1 - 2.0 ** -53, 0), (0.5, 20000001)):
+                at = dev(capi, [u], np.float64)
+                capi.logits_draw(m, base.code(capi, dtype), 1, n, capi.DrawRules(top_k=dev(capi, [k], np.uint32)), tokens, uniforms=at, logprobs=logprobs, kept=kept, workspace=ws)
+                stay = min(k or there, there)
+                rank = int(u * stay)
+                assert (int(tokens.to_host()[0]), int(kept.to_host()[0])) == (3 * rank + 1 if third else rank, stay)
+                assert abs(float(logprobs.to_host()[0]) + np.log(stay)) < 1e-6 * np.log(stay)
 
 
 # ------------------------------------------------------------------------------------------------ route
@@ -135,3 +186,104 @@ def test_route_past_pairs_of_equal_experts(capi, sigmoid, E, groups, kept):  # n
     for k in (1, 2, 3, 8, 13, 16):
         for b in (np.zeros(E, np.float32), np.full(E, 0.25, np.float32)):
             run_route(capi, x, "f32", k, sigmoid=sigmoid, bias=b, groups=groups, kept=kept, top2=k % 2 == 1)
+
+
+@pytest.mark.parametrize("E,k", [(40, 30), (256, 64), (300, 64), (1000, 20)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_route_backward_of_ids_whose_experts_are_closed(capi, sigmoid, E, k):  # noqa: F811
+    rng = np.random.default_rng(E + k)
+    rows = 21
+    x = rng.normal(0, 2, (rows, E)).astype(np.float32)
+    x = np.where(rng.random(x.shape) < 0.4, rng.choice(np.float32([-INF, np.nan]), x.shape), x).astype(np.float32)
+    x[5] = -INF
+    ids = np.stack([rng.permutation(E)[:k] for _ in range(rows)]).astype(np.uint32)
+    ids[rng.random(ids.shape) < 0.1] = INVALID
+    dw = rng.normal(size=(rows, k)).astype(np.float32)
+    for renormalise in (False, True):
+        m, dx = Matrix(capi, x, "f32", 3), Matrix(capi, np.full(x.shape, 9.0), "f32", 1)
+        capi.route_topk_backward(m, capi.F32, rows, E, capi.RouteRules(k, sigmoid=sigmoid, renormalise=renormalise), dev(capi, ids, np.uint32), dev(capi, dw, np.float32), dx,
+                                 row_stride=m.stride, dlogits_stride=dx.stride)
+        want = so.route_backward(m.values, ids, dw, sigmoid, renormalise, 1.0)
+        # as in run_route: exponentials, sums of up to 1,024 and 64 in fp32, over the size of all of the row's gradients
+        base.near(dx.read(), want, np.abs(dw).sum(1, keepdims=True) * (40 + 2 * 10) * 2.0 ** -24 + np.zeros_like(want), "f32")
+
+
+# ------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+class FarRows:
+    """Rows so far apart that the last ones' elements have numbers above 2^32, in memory that nothing else is read from."""
+
+    def __init__(self, capi, values, dtype, stride):
+        bits, self.values = so.to_bits(values, dtype)
+        self.capi, self.dtype, self.stride, self.bits = capi, dtype, stride, bits
+        self.dev = capi.DeviceArray((len(bits) - 1) * stride + bits.shape[1], bits.dtype)
+        self.ptr = self.dev.ptr.value
+        for r in range(len(bits)):
+            self._put(r)
+
+    def _put(self, r):
+        row = np.ascontiguousarray(self.bits[r])
+        assert self.capi.lib().sky_memcpy_h2d(ctypes.c_void_p(self.ptr + r * self.stride * row.itemsize), row.ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(row.nbytes)) == 0
+
+    def read(self):
+        out = np.empty_like(self.bits)
+        for r in range(len(out)):
+            row = np.empty(out.shape[1], out.dtype)
+            assert self.capi.lib().sky_memcpy_d2h(row.ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(self.ptr + r * self.stride * row.itemsize), ctypes.c_size_t(row.nbytes)) == 0
+            out[r] = row
+        return so.from_bits(out, self.dtype)
+
+
+@pytest.mark.parametrize("columns", [100, 40000])
+def test_rows_that_begin_beyond_32_bits(capi, orc, columns):  # noqa: F811
+    rng = np.random.default_rng(29)
+    rows, stride = 4, (1 << 31) - 1
+    x = rng.normal(0, 3, (rows, columns)).astype(np.float32)
+    m, out = FarRows(capi, x, "bf16", stride), FarRows(capi, np.zeros_like(x), "bf16", stride)
+    kw = some_rules(rng, rows, columns, 9, 5, 2)
+    rules = capi.LogitsRules(history=dev(capi, kw["history"], np.uint32), history_columns=9, repetition=dev(capi, kw["rep"], np.float32),
+                             allowed=dev(capi, kw["masks"], np.uint32), allowed_rows=2, allowed_stride=kw["masks"].shape[1], allowed_row=dev(capi, kw["mask_row"], np.uint32))
+    capi.logits_adjust(m, capi.BF16, rows, columns, rules, out, row_stride=stride, out_stride=stride)
+    want, error = so.adjust(m.values, history=kw["history"], rep=kw["rep"], masks=kw["masks"], mask_row=kw["mask_row"])
+    base.near(out.read(), want, error, "bf16")
+    tokens, u = capi.DeviceArray(rows, np.uint32), rng.random(rows)
+    capi.logits_draw(m, capi.BF16, rows, columns, None, tokens, uniforms=dev(capi, u, np.float64), row_stride=stride)
+    assert tokens.to_host().tolist() == [so.draw(m.values[r], u=float(u[r]))[0] for r in range(rows)]
+    if columns <= 1024:
+        ids, w = capi.DeviceArray(rows * 5, np.uint32), capi.DeviceArray(rows * 5, np.float32)
+        for r in (capi.RouteRules(5, sigmoid=True, renormalise=False), capi.RouteRules(5)):
+            capi.route_topk(m, capi.BF16, rows, columns, r, ids, w, row_stride=stride)
+            chosen = ids.to_host().reshape(rows, 5)
+            assert np.array_equal(chosen, so.route(m.values, 5)[0])
+            capi.route_topk_backward(m, capi.BF16, rows, columns, r, ids, w, out, row_stride=stride, dlogits_stride=stride)
+            dw = w.to_host().reshape(rows, 5)
+            want = so.route_backward(m.values, chosen, dw, bool(r.sigmoid), bool(r.renormalise))
+            base.near(out.read(), want, np.full(want.shape, 5 * 60 * 2.0 ** -24), "bf16")
+
+
+# ------------------------------------------------------------------------------------------------ memory
+def test_no_path_of_the_calls_allocates(capi):  # noqa: F811
+    rng = np.random.default_rng(19)
+    g = capi.Graph.upload(np.array([0, 1, 2], np.uint32), np.array([1, 0], np.uint32), None)
+    parts, long, r_in = Matrix(capi, rng.normal(0, 3, (24, 40003)), "f32"), Matrix(capi, rng.normal(0, 3, (300, 21000)), "bf16"), Matrix(capi, rng.normal(0, 2, (50, 300)), "f32")
+    need = capi.logits_draw_workspace(capi.F32, 24, 40003)
+    assert need > 0
+    ws, tokens = capi.DeviceArray(need, np.uint8), capi.DeviceArray(300, np.uint32)
+    ids, w, counts, dx = capi.DeviceArray(200, np.uint32), capi.DeviceArray(200, np.float32), capi.DeviceArray(300, np.uint32), capi.DeviceArray(50 * 300, np.float32)
+    top_p = capi.DrawRules(top_p=dev(capi, np.full(300, 0.9), np.float32))
+    held = capi.LogitsRules(graph=g, states=dev(capi, np.arange(24) % 2, np.uint32))
+
+    def all_calls():
+        capi.logits_draw(parts, capi.F32, 24, 40003, top_p, tokens, seed=1, workspace=ws)
+        capi.logits_draw(long, capi.BF16, 300, 21000, top_p, tokens, seed=1)
+        capi.route_topk(r_in, capi.F32, 50, 300, capi.RouteRules(4), ids, w, counts=counts)
+        capi.route_topk_backward(r_in, capi.F32, 50, 300, capi.RouteRules(4), ids, w, dx)
+        capi.route_topk(r_in, capi.F32, 50, 200, capi.RouteRules(4), ids, w, counts=counts, row_stride=300)
+        capi.logits_adjust(parts, capi.F32, 24, 40003, held, parts)
+        capi.synchronize()
+
+    all_calls()
+    before, _ = capi.mem_info()
+    for _ in range(3):
+        all_calls()
+    assert capi.mem_info()[0] == before
+    g.free()
