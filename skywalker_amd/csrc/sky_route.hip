@@ -850,12 +850,13 @@ int check_route(const char* who, uint32_t rows, uint32_t experts, const sky_rout
    : experts <= 64 ? launch(kernel<T, 4>)                                                 \
    : experts <= 128 ? launch(kernel<T, 8>)                                                \
                     : launch(kernel<T, 16>))
-#define SKY_ROUTE_PIECES(kernel, T)                     \
-  (lanes == 16 ? (pieces <= 1   ? launch(kernel<T, 16, 1>)  \
-                  : pieces <= 2 ? launch(kernel<T, 16, 2>)  \
-                                : launch(kernel<T, 16, 4>)) \
-               : (pieces <= 2 ? launch(kernel<T, 64, 2>)    \
-                              : launch(kernel<T, 64, 4>)))
+// (16-bit rows have two pieces a lane at most)
+#define SKY_ROUTE_PIECES(kernel, T)                                           \
+  (lanes == 16 ? (pieces <= 1   ? launch(kernel<T, 16, 1>)                    \
+                  : pieces <= 2 ? launch(kernel<T, 16, 2>)                    \
+                                : launch(kernel<T, 16, sizeof(T) == 4 ? 4 : 2>)) \
+               : (pieces <= 2 ? launch(kernel<T, 64, 2>)                      \
+                              : launch(kernel<T, 64, sizeof(T) == 4 ? 4 : 2>)))
 #define SKY_ROUTE_LAUNCH(PER, kernel)       \
   (dtype == SKY_F32 ? PER(kernel, float)    \
    : dtype == SKY_F16 ? PER(kernel, _Float16) \
@@ -952,7 +953,7 @@ extern "C" int sky_route_topk_backward(const void* logits, int dtype, uint32_t r
   const hipStream_t st = (hipStream_t)stream;
   // up to 256 experts four rows a wavefront, more one
   const uint32_t lanes = experts <= QUAD_EXPERTS ? 16 : 64, per_block = 64 / lanes * ROUTE_WAVES;
-  const uint32_t pieces = (uint32_t)((experts * dtype_size(dtype) + 16 * lanes - 1) / (16 * lanes));  // a lane: up to 4
+  const uint32_t pieces = (uint32_t)((experts * dtype_size(dtype) + 16 * lanes - 1) / (16 * lanes));  // a lane: up to 4 of fp32, 2 of 16 bits
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((rows + per_block - 1) / per_block), dim3(64 * ROUTE_WAVES), 0, st, a); };
   SKY_ROUTE_LAUNCH(SKY_ROUTE_PIECES, route_backward_kernel);
   return check_launch();
