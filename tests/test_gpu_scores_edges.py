@@ -287,3 +287,89 @@ def test_no_path_of_the_calls_allocates(capi):  # noqa: F811
         all_calls()
     assert capi.mem_info()[0] == before
     g.free()
+
+
+# ------------------------------------------------------------------------------------------------ together
+def test_walk_in_place_with_the_paths_so_far_as_history(capi, orc):  # noqa: F811
+    rng = np.random.default_rng(31)
+    xadj, adjncy = orc.rmat_csr(11, 10, 5)
+    V, N, steps, seed = 2048, 60, 5, 77
+    g = capi.Graph.upload(xadj, adjncy, None)
+    paths = dev(capi, rng.integers(0, V, (N, steps + 1)), np.uint32)  # columns that are not drawn yet hold anything
+    rep, t = rng.uniform(1.0, 1.4, N).astype(np.float32), rng.uniform(0.5, 1.5, N).astype(np.float32)
+    d_rep, draw = dev(capi, rep, np.float32), capi.DrawRules(temperature=dev(capi, t, np.float32))
+    device = [Matrix(capi, rng.normal(0, 2, (N, V)).astype(np.float32), "bf16", 1, 1) for _ in range(steps)]
+    hip = base.Hip()
+    side = hip.stream()
+    capi.synchronize()
+
+    class Column:
+        def __init__(self, at):
+            self.ptr = paths.ptr.value + 4 * at
+
+    for i in range(steps):
+        rules = capi.LogitsRules(history=paths, history_columns=i + 1, history_stride=steps + 1, repetition=d_rep, graph=g, states=Column(i), states_stride=steps + 1)
+        capi.logits_adjust(device[i], capi.BF16, N, V, rules, device[i], row_stride=V + 1, out_stride=V + 1, stream=side)
+        capi.logits_draw(device[i], capi.BF16, N, V, draw, Column(i + 1), seed=seed, step=i, tokens_stride=steps + 1, row_stride=V + 1, stream=side)
+    capi.synchronize()
+    got = paths.to_host((N, steps + 1))
+    for i in range(steps):
+        want, error = so.adjust(device[i].values, history=got[:, :i + 1], rep=rep, xadj=xadj, adjncy=adjncy, states=got[:, i])
+        now = device[i].read()
+        base.near(now, want, error, "bf16")
+        for r in range(N):
+            tok = so.draw(now[r], float(t[r]), u=so.philox_uniform(orc, seed, r, i))[0]
+            assert got[r, i + 1] == (INVALID if tok is None else tok)
+    hip.hipStreamDestroy(side)
+    g.free()
+
+
+def test_other_paths_in_a_graph(capi):  # noqa: F811
+    # rows held to a graph, long 16-bit rows by two kernels, more than 256 experts
+    rng = np.random.default_rng(37)
+    rows, columns, E = 270, 21000, 400
+    degs = rng.integers(0, 1500, columns) * (rng.random(columns) < 0.05)
+    xadj = np.concatenate([[0], np.cumsum(degs)]).astype(np.uint32)
+    g = capi.Graph.upload(xadj, rng.integers(0, columns, int(xadj[-1]), dtype=np.uint32), None)
+    x, r_in = Matrix(capi, rng.normal(0, 3, (rows, columns)), "bf16"), Matrix(capi, rng.normal(0, 2, (rows, E)), "bf16")
+    held = capi.LogitsRules(graph=g, states=dev(capi, rng.choice(np.append(np.flatnonzero(degs), INVALID), rows), np.uint32))
+    draw = capi.DrawRules(top_p=dev(capi, np.full(rows, 0.8), np.float32), temperature=dev(capi, rng.choice([0.0, 0.5, 1.0], rows), np.float32))
+    route = capi.RouteRules(6, bias=dev(capi, rng.uniform(-0.1, 0.1, E), np.float32))
+
+    def outputs():
+        z = lambda n, d: dev(capi, np.zeros(n), d)  # noqa: E731
+        return dict(y=z(rows * columns, np.uint16), some=z(rows, np.uint32), all=z(rows, np.uint32), lp=z(rows, np.float32), ids=z(rows * 6, np.uint32), w=z(rows * 6, np.float32), counts=z(E, np.uint32),
+                    dx=z(rows * E, np.uint16))
+
+    def step(o, s):
+        capi.logits_draw(x, capi.BF16, rows, columns, draw, o["all"], seed=3, step=1, logprobs=o["lp"], stream=s)
+        capi.logits_adjust(x, capi.BF16, rows, columns, held, o["y"], stream=s)
+        capi.logits_draw(o["y"], capi.BF16, rows, columns, draw, o["some"], seed=3, step=2, stream=s)
+        capi.route_topk(r_in, capi.BF16, rows, E, route, o["ids"], o["w"], counts=o["counts"], stream=s)
+        capi.route_topk_backward(r_in, capi.BF16, rows, E, route, o["ids"], o["w"], o["dx"], stream=s)
+
+    hip, eager, captured = base.Hip(), outputs(), outputs()
+    side, graph, ready = hip.stream(), ctypes.c_void_p(), ctypes.c_void_p()
+    capi.synchronize()
+    step(eager, None)
+    capi.synchronize()
+    hip.hipStreamBeginCapture(side, 0)
+    step(captured, side)
+    hip.hipStreamEndCapture(side, ctypes.byref(graph))
+    hip.hipGraphInstantiate(ctypes.byref(ready), graph, None, None, ctypes.c_size_t(0))
+    for _ in range(4):
+        for m in (x, r_in):
+            fresh = so.to_bits(rng.normal(0, 2, m.rows * m.columns).astype(np.float32), "bf16")[0]
+            hip.hipMemcpy(m.dev.ptr, fresh.ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(fresh.nbytes), 1)
+        capi.synchronize()
+        hip.hipGraphLaunch(ready, side)
+        capi.synchronize()
+        step(eager, None)
+        capi.synchronize()
+        for name in eager:
+            assert np.array_equal(eager[name].to_host(), captured[name].to_host()), name
+        assert (eager["some"].to_host() == INVALID).any() and (eager["some"].to_host() != INVALID).any()
+    hip.hipGraphExecDestroy(ready)
+    hip.hipGraphDestroy(graph)
+    hip.hipStreamDestroy(side)
+    g.free()
