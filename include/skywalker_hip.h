@@ -294,7 +294,8 @@ int sky_logits_adjust(const void* logits, int dtype, uint32_t rows, uint32_t col
  * At most 2^26 columns (SKY_ERR_LIMIT).
  * workspace: sky_logits_draw_workspace says how many bytes a draw of such a matrix can make use of (0: none), aligned to 16; nothing need
  * be in them, two calls that may run at the same time have one workspace each, and a captured graph keeps its own.  With it several
- * workgroups share each of a few long fp32 rows; NULL: every row is drawn from by one workgroup.  The ids are the same. */
+ * workgroups share each of a few long fp32 rows; NULL: every row is drawn from by one workgroup.  The ids are the same.  It is for rows without
+ * top-k (40 of 100,003 columns by top-p 50 us instead of 95); a call whose rows all have one is 2 us faster without, 8 us for a top-k above 128. */
 typedef struct sky_draw_rules {
   const float* temperature;
   const uint32_t* top_k;

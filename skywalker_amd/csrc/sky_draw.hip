@@ -1743,12 +1743,15 @@ __global__ __launch_bounds__(SHORT_THREADS, 4) void draw_short_kernel(DrawArgs a
 // CU.  16-bit logits are the exception: a long row of which many entries can stay is drawn from by value, which takes a CU.  (us, 1024 /
 // 256 threads: 2,000 x 8,000 bf16 by top-p 146 / 76, top-k of 50 80 / 23; 1,000 x 20,000 by top-p 82 / 74, 400 x 30,000 42 / 63,
 // 256 x 131,072 37 / 253; 400 x 100,000 top-k of 50 33 / 25; fp32 100 x 20,000 by top-p 46 / 39, 600 x 100,000 322 / 244,
-// 40 x 100,003 top-k of 40 18 / 23.)
+// 40 x 100,003 top-k of 40 18 / 23.)  The lengths come from 100 rows and more.  With fewer rows than CUs they do not hold for all: 40 x 20,000 bf16
+// by top-p 21 / 38, by top-k of 300 and top-p 20 / 55, by top-k of 50 11 / 11, 40 x 5,000 19 / 21, 22 / 30 and 13 / 9, 40 x 1,000 22 / 16, 21 / 23
+// and 20 / 9; fp32 40 x 20,000 44 / 40, 23 / 59 and 15 / 12, 40 x 32,768 52 / 52, 23 / 80 and 15 / 14, 40 x 5,000 36 / 21, 23 / 31 and 14 / 9.  One row
+// and 200 are as 40 are.  So a few rows of 16 bits above some 5,000, and those by a top-k of 129 to 512, would be drawn from faster by 1024 threads.
 constexpr uint32_t SHORT_ROW_16 = 20480, SHORT_ROW_32 = 32768, MANY_ROWS = 256;
 // Parts of a row: two workgroups a CU, of at least 4,096 columns each, eight and more.  What rows of few candidates lose is the launches of
 // kernels that have nothing to do with them.  (us, a workgroup a row / in parts, fp32: 8 x 131,072 by top-p 114 / 48, top-k of 50
 // 19 / 21, of 400 34 / 42; 40 x 100,003 by top-p 95 / 50, top-k of 40 19 / 22; 128 x 100,003, by four, 107 / 95 and 27 / 31.  16-bit rows, whose values are
-// counted: 65,536 by top-k of 50 11 / 17.)
+// counted: 65,536 by top-k of 50 11 / 17.  40 x 100,003, every row its own settings: 21 / 23, and 100-130 / 46 if one row of the 40 has no top-k.)
 Parts parts_of(size_t size, uint32_t rows, uint32_t columns, void* workspace) {
   Parts p{};
   if (size != 4 || !rows || columns <= SHORT_ROW_32) return p;
