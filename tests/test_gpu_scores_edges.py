@@ -260,6 +260,53 @@ def test_rows_that_begin_beyond_32_bits(capi, orc, columns):  # noqa: F811
             base.near(out.read(), want, np.full(want.shape, 5 * 60 * 2.0 ** -24), "bf16")
 
 
+# ------------------------------------------------------------------------------------------------ the largest calls
+@pytest.mark.parametrize("by_graph", [False, True])
+def test_adjust_of_the_widest_row(capi, by_graph):  # noqa: F811
+    n, one = 1 << 30, 0x3C003C00  # 1.0 in both halves
+    x, out = capi.DeviceArray(n // 2, np.uint32, fill=one), capi.DeviceArray(n // 2, np.uint32, fill=0)
+    V = 9000  # a graph's neighbours are among its vertices
+    ids = np.array([0, 7, 4095, 4096, 5000, V - 9, V - 1] if by_graph else [0, 7, 4095, 4096, n // 2, n - 9, n - 1], np.uint32)
+    xadj = np.full(V + 1, len(ids), np.uint32)
+    xadj[0] = 0
+    g = capi.Graph.upload(xadj, ids, None) if by_graph else None
+    rules = capi.LogitsRules(history=dev(capi, ids[1::2], np.uint32), history_columns=3, presence=dev(capi, [0.5], np.float32), bias_offsets=dev(capi, [0, len(ids)], np.uint32),
+                             bias_ids=dev(capi, ids, np.uint32), bias_values=dev(capi, np.arange(len(ids)) + 1.0, np.float32), bias_count=len(ids),
+                             graph=g, states=dev(capi, [0], np.uint32) if by_graph else None)
+    capi.logits_adjust(x, capi.F16, 1, n, rules, out)
+    want = 2.0 + np.arange(len(ids)) - 0.5 * (np.arange(len(ids)) % 2)
+    for at in ids.tolist() + [n // 2, n - 1]:
+        lo = min(max(at - 40, 0), n - 80)
+        near = np.empty(80, np.float16)
+        assert capi.lib().sky_memcpy_d2h(near.ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(out.ptr.value + 2 * lo), ctypes.c_size_t(160)) == 0
+        here = {int(i) - lo: v for i, v in zip(ids, want) if lo <= i < lo + 80}
+        assert near.tolist() == [here.get(i, -INF if by_graph else 1.0) for i in range(80)], at
+    if g:
+        g.free()
+
+
+def test_adjust_and_route_of_the_most_rows(capi):  # noqa: F811
+    rows = 1 << 25
+    x = np.random.default_rng(41).integers(-1000, 1000, (rows, 2)).astype(np.float16)
+    m, y = capi.DeviceArray.from_host(x), capi.DeviceArray(rows * 2, np.float16)
+    capi.logits_adjust(m, capi.F16, rows, 2, capi.LogitsRules(allowed=dev(capi, [1, 2, 3], np.uint32), allowed_rows=3, allowed_row=dev(capi, np.arange(rows) % 3, np.uint32)), y)
+    want = x.copy()
+    want[0::3, 1] = want[1::3, 0] = -INF
+    assert np.array_equal(y.to_host().reshape(rows, 2), want)
+    ids, w, counts = capi.DeviceArray(rows, np.uint32), capi.DeviceArray(rows, np.float32), capi.DeviceArray(2, np.uint32)
+    capi.route_topk(y, capi.F16, rows, 2, capi.RouteRules(1), ids, w, counts=counts)
+    chosen = (want[:, 1] > want[:, 0]).astype(np.uint32)
+    assert np.array_equal(ids.to_host(), chosen) and counts.to_host().tolist() == np.bincount(chosen, minlength=2).tolist()
+    assert (w.to_host() == 1.0).all()
+    capi.route_topk_backward(y, capi.F16, rows, 2, capi.RouteRules(1, sigmoid=True, renormalise=False), ids, w, m)
+    z = want.astype(np.float32).max(1)
+    s = 1.0 / (1.0 + np.exp(-np.abs(z)))
+    got, at = m.to_host().reshape(rows, 2), np.arange(rows)
+    assert (got[at, 1 - chosen] == 0).all()
+    # three exponentials' worth of fp32 roundings, one to 16 bits
+    assert (np.abs(got[at, chosen].astype(np.float64) - s * (1.0 - s)) <= s * (1.0 - s) * (2.0 ** -11 + 2.0 ** -20) + 2.0 ** -23).all()
+
+
 # ------------------------------------------------------------------------------------------------ memory
 def test_no_path_of_the_calls_allocates(capi):  # noqa: F811
     rng = np.random.default_rng(19)
