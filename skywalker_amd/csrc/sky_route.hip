@@ -2,9 +2,9 @@
 //   score    s_e = exp(x_e - max) / sum, or 1 / (1 + exp(-x_e))
 //   choice   by s_e + b_e, the largest first, equal ones by number.  Both scores ascend with the logit, so without a bias and
 //            without pairs of experts the choice goes by the logits themselves, exactly.  Else it is made from scores in fp32, whose error
-//            has a bound; where two of those that it hangs on (neighbours among the k + 1 best, what is as near to the last of them, the last group that stays and the
-//            first that does not) are nearer than that and not alike, the row is chosen again in fp64: one expert more or less is no
-//            rounding error.  (32,768 rows of 256, 8 of 4 of 8 groups: all in fp64 96 us.)
+//            has a bound; where two of those that it hangs on (neighbours among the k + 1 best, what is as near to the last chosen, the
+//            last group that stays and the first that does not) are nearer than that and not alike, the row is chosen again in fp64: one
+//            expert more or less is no rounding error.  (32,768 rows of 256, 8 of 4 of 8 groups: all in fp64 96 us.)
 //   weights  w_j = scale * s_j, renormalised scale * s_j / sum of the k chosen.  Renormalised, the sum over all experts drops out of
 //            softmax scores, and sigmoid scores are taken relative to the largest of the chosen (their logarithms
 //            are at hand), so that a row of tiny scores keeps its shares.  In fp64, for as many rows at once as the chosen fill a wavefront.
